@@ -18,6 +18,8 @@ from astrai_b200.ops.backend import (
     attn_backend,
     get_backend,
 )
+from astrai_b200.ops.kv import KVCache
+from astrai_b200.ops.kv4 import copy_pages_, kv4_append_, kv4_decode, kv4_decode_workspace, kv4_gather
 from astrai_b200.ops.native import KERNEL_NAMES, kernel_available as is_available
 from astrai_b200.ops.functional import (
     adamw_,
@@ -42,9 +44,9 @@ from astrai_b200.ops.functional import (
 __all__ = [
     "adamw_", "add_rms_norm", "apply_rotary_emb", "assume_loss_grad", "attention", "AttentionBackend",
     "AttentionBackendFactory", "ATTN_BACKEND", "attn_backend", "attn_decode", "attn_paged_decode", "attn_paged_prefill",
-    "attn_prefill", "clip_coef", "cross_entropy", "CudaBackend", "DelayedScaling", "dense_attention", "DynamicScaling",
+    "attn_prefill", "clip_coef", "copy_pages_", "cross_entropy", "CudaBackend", "DelayedScaling", "dense_attention", "DynamicScaling",
     "embedding", "flash_attn_available", "FlashAttnBackend", "fp8", "fp8_autocast", "FP8Format", "gemm", "get_backend",
-    "is_available", "KERNEL_NAMES", "linear", "linear_cross_entropy", "linear_token_logprobs", "loss_denominator",
+    "is_available", "KERNEL_NAMES", "KVCache", "kv4_append_", "kv4_decode", "kv4_decode_workspace", "kv4_gather", "linear", "linear_cross_entropy", "linear_token_logprobs", "loss_denominator",
     "native", "qkv_rope", "reference", "repeat_kv", "rms_norm", "rotary", "rotary_emb", "sumsq", "swiglu",
     "swiglu_fused", "Tcgen05Backend", "TensorLayout", "TorchNativeBackend",
 ]

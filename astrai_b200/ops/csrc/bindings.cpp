@@ -362,6 +362,172 @@ void paged_decode_append_(const Tensor& q, const Tensor& k_new, const Tensor& v_
                     &k_new, &v_new);
 }
 
+// ---- 4-bit KV cache ----
+struct Kv4Pools {
+  int64_t slots, heads, dim;
+};
+
+// codes uint8 [slots, heads, D / 2], meta bf16 [slots, heads, D / 32, 2], the same shapes for keys and values.
+Kv4Pools kv4_check(const char* what, const Tensor& k_codes, const Tensor& k_meta, const Tensor& v_codes, const Tensor& v_meta) {
+  for (const Tensor* t : {&k_codes, &k_meta, &v_codes, &v_meta})
+    TORCH_CHECK(t->is_cuda() && t->is_contiguous() && t->device() == k_codes.device(), what, ": the pools must be contiguous CUDA tensors of one device");
+  TORCH_CHECK(k_codes.scalar_type() == at::kByte && v_codes.scalar_type() == at::kByte && k_codes.dim() == 3 && v_codes.sizes() == k_codes.sizes(),
+              what, ": k_codes / v_codes must be uint8 [slots, heads, head_dim / 2]");
+  const Kv4Pools p{k_codes.size(0), k_codes.size(1), 2 * k_codes.size(2)};
+  TORCH_CHECK(p.dim == 32 || p.dim == 64 || p.dim == 128 || p.dim == 256, what, ": head_dim must be 32, 64, 128 or 256, got ", p.dim);
+  for (const Tensor* t : {&k_meta, &v_meta})
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 4 && t->size(0) == p.slots && t->size(1) == p.heads &&
+                    t->size(2) == p.dim / 32 && t->size(3) == 2,
+                what, ": k_meta / v_meta must be bf16 [slots, heads, head_dim / 32, 2]");
+  for (const Tensor* t : {&k_codes, &k_meta, &v_codes, &v_meta})
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0, what, ": the pools must be 16-byte aligned");
+  return p;
+}
+
+void kv4_check_loc(const char* what, const Tensor& loc, const Tensor& pool) {
+  TORCH_CHECK(loc.is_cuda() && loc.device() == pool.device() && loc.is_contiguous() && loc.dim() == 1 &&
+                  (loc.scalar_type() == at::kInt || loc.scalar_type() == at::kLong),
+              what, ": loc must be a contiguous int32 or int64 vector on the pools' device");
+}
+
+// Rows that the kernels can read in place: unit inner stride, every row on a 16-byte boundary.
+Tensor kv4_rows(const Tensor& t) {
+  const bool ok = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  return ok ? t : t.contiguous();
+}
+
+void kv4_check_new(const char* what, const Tensor& k, const Tensor& v, const Tensor& pool, int64_t tokens, const Kv4Pools& p) {
+  TORCH_CHECK(k.device() == pool.device() && v.device() == pool.device() && k.scalar_type() == at::kBFloat16 &&
+                  v.scalar_type() == at::kBFloat16 && k.dim() == 3 && v.sizes() == k.sizes() && k.size(0) == tokens &&
+                  k.size(1) == p.heads && k.size(2) == p.dim,
+              what, ": k / v must be bf16 [", tokens, ", ", p.heads, ", ", p.dim, "] on the pools' device");
+}
+
+void kv4_append_(const Tensor& k, const Tensor& v, Tensor& k_codes, Tensor& k_meta, Tensor& v_codes, Tensor& v_meta, const Tensor& loc) {
+  const Kv4Pools p = kv4_check("kv4_append_", k_codes, k_meta, v_codes, v_meta);
+  kv4_check_loc("kv4_append_", loc, k_codes);
+  kv4_check_new("kv4_append_", k, v, k_codes, loc.numel(), p);
+  const c10::cuda::CUDAGuard guard(k_codes.device());
+  const Tensor kr = kv4_rows(k), vr = kv4_rows(v);
+  count();
+  const int rc = ab::kv4_append(kr.data_ptr(), vr.data_ptr(), k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(), v_meta.data_ptr(),
+                                loc.data_ptr(), loc.scalar_type() == at::kLong, loc.numel(), (int)p.heads, (int)p.dim, p.slots, kr.stride(0),
+                                kr.stride(1), vr.stride(0), vr.stride(1), stream());
+  TORCH_CHECK(rc == 0, "kv4_append_ launch failed with code ", rc);
+}
+
+std::tuple<Tensor, Tensor> kv4_gather(const Tensor& k_codes, const Tensor& k_meta, const Tensor& v_codes, const Tensor& v_meta, const Tensor& loc) {
+  const Kv4Pools p = kv4_check("kv4_gather", k_codes, k_meta, v_codes, v_meta);
+  kv4_check_loc("kv4_gather", loc, k_codes);
+  const c10::cuda::CUDAGuard guard(k_codes.device());
+  Tensor k = at::empty({loc.numel(), p.heads, p.dim}, k_meta.options()), v = at::empty_like(k);
+  count();
+  const int rc = ab::kv4_gather(k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(), v_meta.data_ptr(), loc.data_ptr(),
+                                loc.scalar_type() == at::kLong, k.data_ptr(), v.data_ptr(), loc.numel(), (int)p.heads, (int)p.dim, p.slots, stream());
+  TORCH_CHECK(rc == 0, "kv4_gather launch failed with code ", rc);
+  return {k, v};
+}
+
+// Decode attention over the 4-bit pools; see kv4_decode in launchers.h.  splits = 0: chosen from max_len.  Scratch: all
+// three tensors or none (allocated for the call).
+void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_codes, Tensor& v_meta, const Tensor& req_to_token,
+                 const Tensor& req_pool_indices, const Tensor& seq_lens, const std::optional<Tensor>& k_new, const std::optional<Tensor>& v_new,
+                 double scale, int64_t max_len, int64_t splits, const std::optional<Tensor>& o_part_, const std::optional<Tensor>& ml_part_,
+                 const std::optional<Tensor>& counters_, Tensor& out) {
+  const Kv4Pools p = kv4_check("kv4_decode", k_codes, k_meta, v_codes, v_meta);
+  const auto dev = k_codes.device();
+  TORCH_CHECK(q_.device() == dev && q_.scalar_type() == at::kBFloat16 && q_.dim() == 3 && q_.size(2) == p.dim,
+              "kv4_decode: q must be bf16 [batch, heads, ", p.dim, "] on the pools' device");
+  const int64_t B = q_.size(0), Hq = q_.size(1), D = p.dim, Hkv = p.heads;
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv >= 1 && Hq / Hkv <= 8, "kv4_decode: 1 to 8 query heads per kv head, got ", Hq, " over ", Hkv);
+  TORCH_CHECK(req_to_token.device() == dev && req_to_token.is_contiguous() && req_to_token.dim() == 2 && req_to_token.scalar_type() == at::kInt,
+              "kv4_decode: req_to_token must be a contiguous int32 [rows, positions] tensor on the pools' device");
+  TORCH_CHECK(req_pool_indices.device() == dev && req_pool_indices.is_contiguous() && req_pool_indices.scalar_type() == at::kInt &&
+                  req_pool_indices.dim() == 1 && req_pool_indices.size(0) == B && seq_lens.device() == dev && seq_lens.is_contiguous() &&
+                  seq_lens.scalar_type() == at::kLong && seq_lens.dim() == 1 && seq_lens.size(0) == B,
+              "kv4_decode: req_pool_indices must be int32 [batch] and seq_lens int64 [batch], on the pools' device");
+  TORCH_CHECK(out.device() == dev && out.is_contiguous() && out.scalar_type() == at::kBFloat16 && out.sizes() == q_.sizes(),
+              "kv4_decode: out must be a contiguous bf16 tensor of q's shape");
+  TORCH_CHECK(k_new.has_value() == v_new.has_value(), "kv4_decode: k_new and v_new come together");
+  if (k_new) kv4_check_new("kv4_decode", *k_new, *v_new, k_codes, B, p);
+  TORCH_CHECK(B <= 65535 && req_to_token.size(0) <= INT32_MAX && req_to_token.size(1) <= INT32_MAX, "kv4_decode: batch or table too large");
+  TORCH_CHECK(B == 0 || (req_to_token.size(0) > 0 && req_to_token.size(1) > 0), "kv4_decode: req_to_token is empty");
+  const c10::cuda::CUDAGuard guard(dev);
+  const int given = o_part_.has_value() + ml_part_.has_value() + counters_.has_value();
+  TORCH_CHECK(given == 0 || given == 3, "kv4_decode: the workspace is three tensors (o_part, ml_part, counters)");
+  constexpr int64_t kMaxSplits = 32;
+  const int64_t limit = given ? o_part_->dim() == 4 ? o_part_->size(2) : 0 : kMaxSplits;
+  if (splits <= 0) splits = ab::kv4_decode_splits((int)B, (int)Hkv, max_len > 0 ? max_len : req_to_token.size(1), (int)limit);
+  TORCH_CHECK(limit >= 1 && splits <= limit, "kv4_decode: ", splits, " splits, the workspace holds ", limit);
+  Tensor o_part, ml_part, counters;
+  if (given) {
+    o_part = *o_part_, ml_part = *ml_part_, counters = *counters_;
+    auto fits = [&](const Tensor& t, int64_t last) {
+      return t.device() == dev && t.is_contiguous() && t.scalar_type() == at::kFloat && t.dim() == 4 && t.size(0) >= B && t.size(1) == Hq &&
+             t.size(2) == limit && t.size(3) == last;
+    };
+    TORCH_CHECK(fits(o_part, D) && fits(ml_part, 2), "kv4_decode: workspace o_part / ml_part must be fp32 [>= batch, heads, splits, head_dim / 2 numbers]");
+    TORCH_CHECK(counters.device() == dev && counters.is_contiguous() && counters.scalar_type() == at::kInt && counters.numel() >= B * Hkv,
+                "kv4_decode: workspace counters must be int32 [>= batch * kv_heads], zero before the first call");
+  } else {
+    const auto f32 = q_.options().dtype(at::kFloat);
+    o_part = at::empty({B, Hq, splits, D}, f32), ml_part = at::empty({B, Hq, splits, 2}, f32);
+    counters = at::zeros({B * Hkv}, q_.options().dtype(at::kInt));
+  }
+  const Tensor q = q_.is_contiguous() && (reinterpret_cast<uintptr_t>(q_.data_ptr()) & 15) == 0 ? q_ : q_.clone(at::MemoryFormat::Contiguous);
+  auto whole = [](const Tensor& t) {
+    return t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+  };
+  const Tensor kn = k_new ? whole(*k_new) : Tensor(), vn = v_new ? whole(*v_new) : Tensor();
+  if (B == 0) return;
+  count();
+  const int rc = ab::kv4_decode(q.data_ptr(), k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(), v_meta.data_ptr(),
+                                req_to_token.data_ptr<int>(), req_pool_indices.data_ptr<int>(), (const long long*)seq_lens.data_ptr<int64_t>(),
+                                k_new ? kn.data_ptr() : nullptr, v_new ? vn.data_ptr() : nullptr, o_part.data_ptr<float>(),
+                                ml_part.data_ptr<float>(), counters.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hq, (int)Hkv, (int)D,
+                                (int)req_to_token.size(1), (int)req_to_token.size(0), p.slots, (float)scale, (int)splits,
+                                (int)o_part.size(2), stream());
+  TORCH_CHECK(rc == 0, "kv4_decode launch failed with code ", rc);
+}
+
+// Page dst[i] of every layer of every pool [layers, slots, ...] becomes a copy of page src[i].
+void copy_pages_(at::TensorList pools, at::IntArrayRef src, at::IntArrayRef dst, int64_t page_size) {
+  using ab::PageCopies;
+  TORCH_CHECK_VALUE(!pools.empty() && pools.size() <= (size_t)PageCopies::kPools, "copy_pages_: 1 to ", (int)PageCopies::kPools, " pools");
+  TORCH_CHECK_VALUE(page_size >= 1 && src.size() == dst.size(), "copy_pages_: page_size >= 1, as many sources as destinations");
+  const auto dev = pools[0].device();
+  for (const Tensor& t : pools)
+    TORCH_CHECK(t.is_cuda() && t.device() == dev && t.is_contiguous() && t.dim() >= 2 && t.size(0) == pools[0].size(0) && t.size(1) == pools[0].size(1),
+                "copy_pages_: the pools must be contiguous CUDA tensors [layers, slots, ...] of one device and as many layers and slots each");
+  const int64_t layers = pools[0].size(0), pages = pools[0].size(1) / page_size;
+  TORCH_CHECK_VALUE(pages <= INT32_MAX, "copy_pages_: too many pages");
+  std::vector<bool> taken(pages, false);
+  for (int64_t d : dst) {
+    TORCH_CHECK_VALUE(d >= 0 && d < pages, "copy_pages_: page ", d, " is outside the pool of ", pages, " pages");
+    TORCH_CHECK_VALUE(!taken[d], "copy_pages_: page ", d, " is written twice");
+    taken[d] = true;
+  }
+  for (int64_t s : src) {
+    TORCH_CHECK_VALUE(s >= 0 && s < pages, "copy_pages_: page ", s, " is outside the pool of ", pages, " pages");
+    TORCH_CHECK_VALUE(!taken[s], "copy_pages_: page ", s, " is both read and written");
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  PageCopies c;
+  for (size_t i = 0; i < pools.size(); ++i) {
+    const int64_t slot = pools[i].size(1) ? (int64_t)pools[i].element_size() * (pools[i].numel() / std::max<int64_t>(1, layers * pools[i].size(1))) : 0;
+    c.base[i] = pools[i].data_ptr();
+    c.page_bytes[i] = slot * page_size;
+    c.layer_bytes[i] = slot * pools[i].size(1);
+  }
+  for (size_t start = 0; start < src.size(); start += PageCopies::kPairs) {
+    const int n = (int)std::min<size_t>(PageCopies::kPairs, src.size() - start);
+    for (int i = 0; i < n; ++i) c.src[i] = (int)src[start + i], c.dst[i] = (int)dst[start + i];
+    count();
+    const int rc = ab::copy_pages(c, n, (int)layers, (int)pools.size(), stream());
+    TORCH_CHECK(rc == 0, "copy_pages_ launch failed with code ", rc);
+  }
+}
+
 // q [Tq, Hq, D], k / v [Tk, Hkv, D] packed along tokens (a dense [B,S,H,D] batch is the same memory).
 std::tuple<Tensor, Tensor> flash_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& cu_q,
                                      const c10::optional<Tensor>& cu_k, int64_t batch, int64_t sq, int64_t sk,
@@ -1107,6 +1273,10 @@ TORCH_LIBRARY(astrai_b200, m) {
   m.def("comm_wait_flags_(Tensor local_flags, int kind, int world, int skip_rank, int unit, int max_units, int epoch, float timeout_s) -> ()", &comm_wait_flags_);
   m.def("kernel_status_reset(Tensor like) -> ()", &kernel_status_reset);
   m.def("flash_fwd(Tensor q, Tensor k, Tensor v, Tensor? cu_q, Tensor? cu_k, int batch, int sq, int sk, int max_q, bool causal, float scale) -> (Tensor, Tensor)", &flash_fwd);
+  m.def("kv4_append_(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor loc) -> ()", &kv4_append_);
+  m.def("kv4_gather(Tensor k_codes, Tensor k_meta, Tensor v_codes, Tensor v_meta, Tensor loc) -> (Tensor, Tensor)", &kv4_gather);
+  m.def("kv4_decode_(Tensor q, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor req_to_token, Tensor req_pool_indices, Tensor seq_lens, Tensor? k_new, Tensor? v_new, float scale, int max_len, int splits, Tensor? o_part, Tensor? ml_part, Tensor? counters, Tensor(e!) out) -> ()", &kv4_decode_);
+  m.def("copy_pages_(Tensor(a!)[] pools, int[] src, int[] dst, int page_size) -> ()", &copy_pages_);
   m.def("flash_fwd_paged(Tensor q, Tensor k_pool, Tensor v_pool, Tensor cu_q, Tensor cu_k, Tensor table, Tensor rows, int page, int max_q, bool causal, float scale) -> Tensor", &flash_fwd_paged);
   m.def("flash_bwd(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, Tensor? cu_q, Tensor? cu_k, int batch, int sq, int sk, int max_q, int max_k, bool causal, float scale) -> (Tensor, Tensor, Tensor)", &flash_bwd);
   m.def("cp_flash_fwd(Tensor q, Tensor k_full, Tensor v_full, int batch, int chunk, int world, int rank, float scale, int[] kv_src_ptrs, int[] flag_ptrs, int unit, int max_units, int epoch, int n_copy_ctas, Tensor? chunk_state, float timeout_s) -> (Tensor, Tensor)", &cp_flash_fwd);

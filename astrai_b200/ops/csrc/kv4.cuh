@@ -1,0 +1,127 @@
+// The 4-bit KV cache: the format of a row and the arithmetic that writes and reads it (sm_100a).
+//
+// A key or value row of D numbers (D = 32 / 64 / 128 / 256) is held in groups of 32.  A group has a step s and a middle m,
+// both bf16, and 32 codes c of four bits; a number reads back as  m + s * (c - 8).  With lo / hi the group's least and
+// greatest number:
+//   s = bf16((hi - lo) / 15)      m = bf16(lo + 8 s)      c = clamp(round_half_even((x - m) / s), -8, 7) + 8
+// The error of a number is at most s / 2 + 2^-8 |m| (the second part is the rounding of m, not more than the bf16 input's
+// own).  A group whose step is 0 or below 2^-126 holds its least number 32 times; a group with an infinity or a NaN, or
+// one that spreads over 2^120 or more, reads back as NaN (m = NaN, s = 0).
+//
+// Memory: codes [slots, heads, D / 2] bytes, lower half of a byte first; (m, s) [slots, heads, D / 32] words, m in the
+// lower half.  The codes of a row are in the order in which the lanes of the attention kernel take them, so that each of
+// them loads its share of a row at once (D = 128: 16 bytes of a key, 8 bytes of a value):
+//   keys    [quarter of a group: 4][group][8 codes], four groups at a time:  a lane's word is 8 numbers of one group
+//   values  [eighth of a group: 8][group][4 codes]:                          a lane's half word is 4 numbers of one group
+#pragma once
+#include "common.cuh"
+
+namespace ab {
+
+// Where word (group w, quarter t) of a key row is held; where half word (group g, eighth i) of a value row is held.
+template <int D> __host__ __device__ constexpr int kv4_key_word(int w, int t) {
+  constexpr int NG = D / 32;
+  return NG <= 4 ? t * NG + w : (w >> 2) * 16 + t * 4 + (w & 3);
+}
+template <int D> __host__ __device__ constexpr int kv4_value_half(int g, int i) { return i * (D / 32) + g; }
+
+// IEEE single arithmetic that keeps subnormal numbers, whatever the flags of the file: the codes are then the ones of the
+// formulas above, the same on every machine.
+__device__ __forceinline__ float sub_ieee(float a, float b) {
+  float r;
+  asm("sub.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float add_ieee(float a, float b) {
+  float r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_ieee(float a, float b) {
+  float r;
+  asm("min.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_ieee(float a, float b) {
+  float r;
+  asm("max.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fma_ieee(float a, float b, float c) {
+  float r;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float div_ieee(float a, float b) {
+  float r;
+  asm("div.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Eight numbers of a lane -> their eight codes (lowest number in the lowest half byte) and the (m, s) word of the group,
+// which four neighbouring lanes share.  Every lane of the warp takes part.
+__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t& meta) {
+  float lo = x[0], hi = x[0];
+  uint32_t big = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    lo = min_ieee(lo, x[j]);
+    hi = max_ieee(hi, x[j]);
+    big = max(big, __float_as_uint(x[j]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    lo = min_ieee(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_ieee(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+  }
+  const float spread = sub_ieee(hi, lo);
+  if (big >= 0x7f800000u || spread >= 0x1p120f) {
+    meta = 0x00007fffu;  // m = NaN, s = 0
+    return 0x88888888u;
+  }
+  uint32_t s_bits = __bfloat16_as_ushort(__float2bfloat16_rn(div_ieee(spread, 15.f)));
+  if (s_bits < 0x0080u) s_bits = 0;  // below 2^-126
+  const float s = __uint_as_float(s_bits << 16);
+  const float mid = s_bits ? add_ieee(lo, 8.f * s) : lo;
+  const uint32_t m_bits = __bfloat16_as_ushort(__float2bfloat16_rn(mid));
+  const float m = __uint_as_float(m_bits << 16);
+  meta = m_bits | (s_bits << 16);
+  if (!s_bits) return 0x88888888u;
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = min(7, max(-8, __float2int_rn(div_ieee(sub_ieee(x[j], m), s)))) + 8;
+    word |= (uint32_t)c << (4 * j);
+  }
+  return word;
+}
+
+// One row per D / 8 lanes: lane `l` of the row brings its numbers 8 l .. 8 l + 7 (`src`), and the row goes to `codes` /
+// `meta`.  Every lane of the warp takes part; a lane with `live` false stores nothing (and its `src` is not read).
+template <int D>
+__device__ __forceinline__ void kv4_store_row(bool live, bool key, int l, const __nv_bfloat16* src, uint8_t* codes, uint32_t* meta) {
+  constexpr int NG = D / 32;
+  Vec8<__nv_bfloat16> v;
+  v.raw = make_uint4(0, 0, 0, 0);
+  if (live) v.load(src + 8 * l);
+  float x[8];
+  v.unpack(x);
+  uint32_t ms;
+  const uint32_t word = kv4_quantise(x, ms);
+  // a value row's words are made of two half words that two lanes may hold
+  const int base = (threadIdx.x & 31) - l;
+  uint32_t out = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int half = 2 * l + e, i = half / NG, g = half % NG;
+    const uint32_t w = __shfl_sync(0xffffffffu, word, base + g * 4 + (i >> 1));
+    out |= ((i & 1) ? (w >> 16) : (w & 0xffffu)) << (16 * e);
+  }
+  if (!live) return;
+  if (key) reinterpret_cast<uint32_t*>(codes)[kv4_key_word<D>(l >> 2, l & 3)] = word;
+  else reinterpret_cast<uint32_t*>(codes)[l] = out;
+  if ((l & 3) == 0) meta[l >> 2] = ms;
+}
+
+}  // namespace ab

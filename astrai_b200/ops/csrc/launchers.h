@@ -269,4 +269,33 @@ int gemm_skinny_splits(int N, int K, int tok);
 int gemm_skinny(const void* X, const void* W, void* Y, int M, int N, int K, long long ldx, long long ldw, long long ldy,
                 int* status, cudaStream_t st);
 
+// ---- 4-bit KV cache (kv4.cu; the format is described in kv4.cuh) ----
+// codes [n_slots, heads, D / 2] bytes, meta [n_slots, heads, D / 32] words, D in {32, 64, 128, 256}.  Return 0, -3: head
+// dim, -4: too large for one launch, -5: launch error.
+// k / v: bf16 rows with unit inner stride, 16-byte aligned; *_tok / *_head: strides in elements.  loc: int32 or int64 (loc64).
+int kv4_append(const void* k, const void* v, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* loc, bool loc64,
+               long long tokens, int heads, int head_dim, long long n_slots, long long k_tok, long long k_head, long long v_tok,
+               long long v_head, cudaStream_t st);
+// k / v out: bf16 [tokens, heads, D] contiguous.
+int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, const void* loc, bool loc64, void* k,
+               void* v, long long tokens, int heads, int head_dim, long long n_slots, cudaStream_t st);
+int kv4_decode_splits(int batch, int n_kv_heads, long long max_len, int max_splits);
+// Scratch as for paged_decode.  k_new / v_new (both or neither): bf16 [batch, n_kv_heads, D], stored into the slot of the
+// last position first.  Returns also -1: more than 8 query heads per kv head, -2: splits.
+int kv4_decode(const void* q, const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, const int* req_to_token,
+               const int* req_pool_indices, const long long* seq_lens, const void* k_new, const void* v_new, float* o_part, float* ml_part,
+               int* counters, void* out, int batch, int n_q_heads, int n_kv_heads, int head_dim, int max_ctx, int table_rows,
+               long long n_slots, float scale, int splits, int max_splits, cudaStream_t st);
+
+// Page copies of one launch: page dst[i] = page src[i] in every layer of every pool (kv4.cu).  No destination may be a
+// source or occur twice.
+struct PageCopies {
+  static constexpr int kPools = 8, kPairs = 256;
+  void* base[kPools] = {};
+  long long page_bytes[kPools] = {};
+  long long layer_bytes[kPools] = {};
+  int src[kPairs] = {}, dst[kPairs] = {};
+};
+int copy_pages(const PageCopies& c, int pairs, int layers, int pools, cudaStream_t st);
+
 }  // namespace ab

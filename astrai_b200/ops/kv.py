@@ -38,3 +38,15 @@ class KVCache:
     kv_gather_loc: Optional[Tensor] = None
     # tokens per page of the pool (1: slots are not grouped into pages); 8 / 16 / 32 / 64 let prefill read the pool in place
     page_size: int = 1
+    # 4-bit pools (:mod:`astrai_b200.ops.kv4`): k_buffer / v_buffer then hold the codes ``uint8 [layers, slots, kv_heads,
+    # head_dim / 2]`` and these the groups' (m, s) ``bf16 [layers, slots, kv_heads, head_dim / 32, 2]``
+    k_meta: Optional[Tensor] = None
+    v_meta: Optional[Tensor] = None
+
+    @property
+    def four_bit(self) -> bool:
+        return self.k_meta is not None
+
+    def layer_pools(self, layer_id: int):
+        """``(k_codes, k_meta, v_codes, v_meta)`` of one layer of a 4-bit cache."""
+        return self.k_buffer[layer_id], self.k_meta[layer_id], self.v_buffer[layer_id], self.v_meta[layer_id]

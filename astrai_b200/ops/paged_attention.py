@@ -8,6 +8,8 @@ Packed layout: ``q [T, Hq, D]``, ``k / v [T, Hkv, D]`` where the batch is concat
   kernel reads K / V straight from the pool through the slot table; other page sizes (and the contiguous layout's
   page size 1) gather the batch's keys into packed tensors first.  Head dims other than 64 / 128 and explicit masks
   take a per-request SDPA loop.
+* a 4-bit cache (:mod:`astrai_b200.ops.kv4`): decode attends on the codes, prefill stores the new rows, reads the batch's rows
+  back as bf16 and runs the same varlen launch.
 The CPU statement of both is the same gather + softmax and is what the tests compare against
 (semantics of ``TorchNativeBackend`` in the reference, ``astrai/extension/backend/attention.py:443-498``).
 """
@@ -20,11 +22,14 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
-from astrai_b200.ops import flash, native
+from astrai_b200.ops import flash, kv4, native
 from astrai_b200.ops.kv import KVCache
 
 
 def _append(k: Tensor, v: Tensor, cache: KVCache, layer_id: int):
+    if cache.four_bit:
+        kv4.kv4_append_(k, v, *cache.layer_pools(layer_id), cache.out_cache_loc.reshape(-1))
+        return
     kb, vb = cache.k_buffer[layer_id], cache.v_buffer[layer_id]
     loc = cache.out_cache_loc.reshape(-1)
     if k.is_cuda and k.dtype == torch.bfloat16 and kb.dtype == torch.bfloat16 and (kb.shape[1] * kb.shape[2]) % 8 == 0:
@@ -38,6 +43,8 @@ def _append(k: Tensor, v: Tensor, cache: KVCache, layer_id: int):
 
 def _gather_kv(cache: KVCache, layer_id: int, row: int, length: int):
     slots = cache.req_to_token[row, :length].long()
+    if cache.four_bit:
+        return kv4.kv4_gather(*cache.layer_pools(layer_id), slots)
     return cache.k_buffer[layer_id][slots], cache.v_buffer[layer_id][slots]
 
 
@@ -75,7 +82,7 @@ def _lens(cache: KVCache):
 
 def _decode_native_ok(q: Tensor, cache: KVCache) -> bool:
     return (
-        q.is_cuda and q.dtype == torch.bfloat16 and cache.k_buffer.dtype == torch.bfloat16
+        q.is_cuda and q.dtype == torch.bfloat16 and (cache.four_bit or cache.k_buffer.dtype == torch.bfloat16)
         and q.shape[-1] in (32, 64, 128, 256) and cache.decode_o_part is not None and cache.decode_counters is not None
         and q.shape[1] % cache.k_buffer.shape[2] == 0 and 1 <= q.shape[1] // cache.k_buffer.shape[2] <= 8
     )
@@ -95,6 +102,12 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
         # one launch: the step's K / V rows are stored into the pool by the attention kernel itself (the reference fuses
         # its append the same way, csrc/kernels/attention/layout_policies.cuh:221-254)
         b = q.shape[0]
+        if kv_cache.four_bit:
+            out = kv_cache.decode_out[:b] if kv_cache.decode_out is not None else None
+            return kv4.kv4_decode(q, *kv_cache.layer_pools(layer_id), kv_cache.req_to_token, kv_cache.req_pool_indices,
+                                  kv_cache.seq_lens, k_new=k, v_new=v, scale=scale, max_len=kv_cache.max_len,
+                                  splits=kv_cache.decode_splits, out=out,
+                                  workspace=(kv_cache.decode_o_part, kv_cache.decode_ml_part, kv_cache.decode_counters))
         splits = kv_cache.decode_splits or int(torch.ops.astrai_b200.paged_decode_splits(
             b, kv_cache.k_buffer.shape[2], max(kv_cache.max_len, 1), kv_cache.decode_o_part.shape[2]))
         out = kv_cache.decode_out[:b] if kv_cache.decode_out is not None else torch.empty_like(q)
@@ -106,14 +119,22 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
     _append(k, v, kv_cache, layer_id)
     q_lens, kv_lens = _lens(kv_cache)
     page = getattr(kv_cache, "page_size", 1) or 1
-    if (native_on and attn_mask is None and fwd == "prefill" and kv_cache.qo_indptr is not None and page in flash.PAGED_PAGE_SIZES
+    if kv_cache.four_bit:
+        if (native_on and attn_mask is None and fwd == "prefill" and kv_cache.kv_gather_loc is not None
+                and kv_cache.qo_indptr is not None and q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in flash.SUPPORTED_HEAD_DIMS):
+            # the prompt's own rows are read back with the cached ones: a token sees the same numbers of a key whether its
+            # prompt ran in one chunk or several
+            kk, vv = kv4.kv4_gather(*kv_cache.layer_pools(layer_id), kv_cache.kv_gather_loc)
+            return flash.flash_attention_varlen(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens),
+                                                causal=True, scale=scale)
+    elif (native_on and attn_mask is None and fwd == "prefill" and kv_cache.qo_indptr is not None and page in flash.PAGED_PAGE_SIZES
             and flash.supported(q, kv_cache.k_buffer[layer_id], kv_cache.v_buffer[layer_id])):
         # ragged prefill over the paged pool: the kernel walks the slot table itself (no gathered copy of the keys)
         return flash.flash_attention_paged(q, kv_cache.k_buffer[layer_id], kv_cache.v_buffer[layer_id], kv_cache.qo_indptr,
                                            kv_cache.kv_indptr, kv_cache.req_to_token, kv_cache.req_pool_indices, page,
                                            max(q_lens), causal=True, scale=scale)
-    if (native_on and attn_mask is None and fwd == "prefill" and kv_cache.kv_gather_loc is not None and kv_cache.qo_indptr is not None
-            and flash.supported(q, kv_cache.k_buffer[layer_id], kv_cache.v_buffer[layer_id])):
+    if (not kv_cache.four_bit and native_on and attn_mask is None and fwd == "prefill" and kv_cache.kv_gather_loc is not None
+            and kv_cache.qo_indptr is not None and flash.supported(q, kv_cache.k_buffer[layer_id], kv_cache.v_buffer[layer_id])):
         # ragged prefill on the tcgen05 flash kernel: gather this batch's keys / values from the pool (cached prefix
         # included) into packed tensors once, then one varlen launch with lower-right aligned causal masking
         kk = kv_cache.k_buffer[layer_id].index_select(0, kv_cache.kv_gather_loc)
