@@ -203,6 +203,7 @@ def _model_options(fn):
         click.option("--device", default="cuda"),
         click.option("--dtype", type=click.Choice(["bfloat16", "float16", "float32"]), default=None, help="Default: bfloat16 on CUDA, float32 on the CPU."),
         click.option("--cache", type=click.Choice(["paged", "contiguous"]), default="paged", help="KV cache layout."),
+        click.option("--kv_dtype", type=click.Choice(["auto", "int4"]), default="auto", help="Precision of the KV cache."),
         click.option("--backend", type=str, default=None, help="Attention back end (tcgen05, torch_native, or a registered name); default: the process default."),
         click.option("--compare", is_flag=True, default=False, help="Run under tcgen05 and torch_native and print both with their ratio."),
     ]):
@@ -259,7 +260,7 @@ def _sync(device):
 @click.option("--batch_size", type=int, default=8)
 @click.option("--prompt_len", type=int, default=1024)
 @click.option("--trials", type=int, default=5)
-def prefill(preset, ckpt, config_path, device, dtype, cache, backend, compare, batch_size, prompt_len, trials):
+def prefill(preset, ckpt, config_path, device, dtype, cache, kv_dtype, backend, compare, batch_size, prompt_len, trials):
     """Tokens/s of packed prefill forwards through the scheduler's executor."""
     import torch
 
@@ -270,7 +271,7 @@ def prefill(preset, ckpt, config_path, device, dtype, cache, backend, compare, b
     prompts = [torch.randint(2, model.config.vocab_size, (prompt_len,), generator=g).tolist() for _ in range(batch_size)]
     rows = []
     for arm in _arms(backend, compare):
-        sched = _scheduler(model, batch_size, prompt_len + 8, cache, arm)
+        sched = _scheduler(model, batch_size, prompt_len + 8, cache, arm, kv_dtype=kv_dtype)
         times = []
         with sched._backend_context():
             for i in range(trials + 3):
@@ -293,7 +294,7 @@ def prefill(preset, ckpt, config_path, device, dtype, cache, backend, compare, b
 @click.option("--prompt_len", type=int, default=128)
 @click.option("--gen_len", type=int, default=256)
 @click.option("--cuda_graph/--no-cuda_graph", default=True)
-def decode(preset, ckpt, config_path, device, dtype, cache, backend, compare, batch_size, prompt_len, gen_len, cuda_graph):
+def decode(preset, ckpt, config_path, device, dtype, cache, kv_dtype, backend, compare, batch_size, prompt_len, gen_len, cuda_graph):
     """Decode tokens/s through scheduler + sampler (+ CUDA graphs)."""
     import torch
 
@@ -302,7 +303,7 @@ def decode(preset, ckpt, config_path, device, dtype, cache, backend, compare, ba
     prompts = [torch.randint(2, model.config.vocab_size, (prompt_len,), generator=g).tolist() for _ in range(batch_size)]
     rows = []
     for arm in _arms(backend, compare):
-        sched = _scheduler(model, batch_size, prompt_len + gen_len + 8, cache, arm, enable_cuda_graph=cuda_graph)
+        sched = _scheduler(model, batch_size, prompt_len + gen_len + 8, cache, arm, enable_cuda_graph=cuda_graph, kv_dtype=kv_dtype)
         with sched._backend_context():
             sched.run_batch(prompts, max_tokens=8, temperature=0.0)  # warm-up
             _sync(device)
@@ -325,6 +326,7 @@ def decode(preset, ckpt, config_path, device, dtype, cache, backend, compare, ba
 @click.option("--max_batch_size", type=int, default=64)
 @click.option("--max_seq_len", type=int, default=8192)
 @click.option("--kv_cache_tokens", type=int, default=None)
+@click.option("--kv_dtype", type=click.Choice(["auto", "int4"]), default="auto", help="Precision of the KV cache.")
 @click.option("--temperature", type=float, default=0.8)
 @click.option("--top_p", type=float, default=0.95)
 @click.option("--top_k", type=int, default=50)
@@ -336,7 +338,7 @@ def decode(preset, ckpt, config_path, device, dtype, cache, backend, compare, ba
               help="'reference' drives the unmodified reference package (importable as `astrai`, e.g. PYTHONPATH=baseline/_ref) "
                    "with the same request stream.")
 @click.option("--ref_backend", type=str, default="flash", help="Attention backend of the reference arm.")
-def serve(preset, device, n_requests, rate, max_batch_size, max_seq_len, kv_cache_tokens, temperature, top_p, top_k, seed,
+def serve(preset, device, n_requests, rate, max_batch_size, max_seq_len, kv_cache_tokens, kv_dtype, temperature, top_p, top_k, seed,
           time_scale, chunked_prefill, max_prefill_tokens, impl, ref_backend):
     """Continuous-batching load test with a paged KV cache (16-token pages) and the radix prefix cache."""
     import torch
@@ -350,7 +352,7 @@ def serve(preset, device, n_requests, rate, max_batch_size, max_seq_len, kv_cach
     model = build_model(preset, device, torch.bfloat16 if device != "cpu" else torch.float32)
     sched = InferenceScheduler(model, _IdTokenizer(), max_batch_size=max_batch_size, max_seq_len=max_seq_len, page_size=16,
                                kv_cache_tokens=kv_cache_tokens or max_batch_size * 4608, paged=True,
-                               chunked_prefill=chunked_prefill, max_prefill_tokens=max_prefill_tokens)
+                               chunked_prefill=chunked_prefill, max_prefill_tokens=max_prefill_tokens, kv_dtype=kv_dtype)
     reqs = make_requests(n_requests, rate, model.config.vocab_size, seed)
     sched.run_batch([reqs[0]["ids"][:64]], max_tokens=4, temperature=0.0)  # warm-up
     sched.start()
@@ -359,7 +361,7 @@ def serve(preset, device, n_requests, rate, max_batch_size, max_seq_len, kv_cach
     finally:
         sched.stop()
     res.update({"benchmark": "serve", "preset": preset, "rate": rate, "max_batch_size": max_batch_size, "page_size": 16,
-                "chunked_prefill": chunked_prefill, "max_prefill_tokens": max_prefill_tokens,
+                "kv_dtype": kv_dtype, "chunked_prefill": chunked_prefill, "max_prefill_tokens": max_prefill_tokens,
                 "sampling": {"temperature": temperature, "top_p": top_p, "top_k": top_k, "seed": seed}})
     click.echo(json.dumps(res))
 

@@ -12,6 +12,7 @@ from typing import List, Optional
 
 import torch
 
+from astrai_b200.ops import kv4
 from astrai_b200.ops.kv import KVCache  # noqa: F401  (re-exported)
 
 
@@ -48,7 +49,21 @@ class ReqToTokenPool:
 
 
 class KVStorage:
-    def __init__(self, size: int, n_layers: int, n_kv_heads: int, head_dim: int, device, dtype):
+    """The K / V pools.  ``four_bit``: codes and the groups' (m, s) of :mod:`astrai_b200.ops.kv4` instead of ``dtype`` rows."""
+
+    def __init__(self, size: int, n_layers: int, n_kv_heads: int, head_dim: int, device, dtype, four_bit: bool = False):
         self.size = size
+        self.k_meta = self.v_meta = None
+        if four_bit:
+            shape = (n_layers, size, n_kv_heads)
+            self.k_buffer = torch.zeros((*shape, head_dim // 2), device=device, dtype=torch.uint8)
+            self.v_buffer = torch.zeros_like(self.k_buffer)
+            self.k_meta = torch.zeros((*shape, head_dim // kv4.GROUP, 2), device=device, dtype=torch.bfloat16)
+            self.v_meta = torch.zeros_like(self.k_meta)
+            return
         self.k_buffer = torch.zeros((n_layers, size, n_kv_heads, head_dim), device=device, dtype=dtype)
         self.v_buffer = torch.zeros((n_layers, size, n_kv_heads, head_dim), device=device, dtype=dtype)
+
+    def pools(self) -> List[torch.Tensor]:
+        """Every tensor that holds a part of a slot's contents, ``[layers, slots, ...]``."""
+        return [t for t in (self.k_buffer, self.k_meta, self.v_buffer, self.v_meta) if t is not None]

@@ -20,8 +20,11 @@ from astrai_b200.inference.cache.strategy import (
     AllocationStrategy, Allocator, ContiguousStrategy, PagedStrategy, RadixCache, TaskCacheState,
 )
 from astrai_b200.inference.workspace import Q_TILE_ROWS, InferenceWorkspace
+from astrai_b200.ops import kv4
+from astrai_b200.ops.kv4 import copy_pages_
 
 DEFAULT_PAGE_SIZE = 16
+KV_DTYPES = ("auto", "int4")
 
 
 def page_hash(token_ids: List[int], page_idx: int, page_size: int, parent_hash: int = 0) -> int:
@@ -39,7 +42,16 @@ class _BindState:
 
 class PagePool:
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, max_batch_size: int, max_seq_len: int, device,
-                 dtype, page_size: int = 1, n_tokens: Optional[int] = None):
+                 dtype, page_size: int = 1, n_tokens: Optional[int] = None, kv_dtype: str = "auto"):
+        """``kv_dtype``: ``"auto"`` holds keys and values in ``dtype``, ``"int4"`` in 4 bits (:mod:`astrai_b200.ops.kv4`)."""
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {', '.join(KV_DTYPES)}, got {kv_dtype!r}")
+        if kv_dtype == "int4":
+            if head_dim not in kv4.HEAD_DIMS:
+                raise ValueError(f"a 4-bit KV cache needs a head_dim of {', '.join(map(str, kv4.HEAD_DIMS))}, the model has {head_dim}")
+            if torch.device(device).type == "cuda" and dtype != torch.bfloat16:
+                raise ValueError(f"a 4-bit KV cache on a GPU takes bf16 keys and values, the model runs in {dtype}")
+        self.kv_dtype = kv_dtype
         self.page_size, self.max_batch_size, self.max_seq_len = page_size, max_batch_size, max_seq_len
         self.device, self.dtype = torch.device(device), dtype
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
@@ -47,7 +59,7 @@ class PagePool:
         self.n_tokens = max_batch_size * max_seq_len if self.contiguous else (n_tokens // page_size) * page_size
         if self.n_tokens > torch.iinfo(torch.int32).max:
             raise ValueError("KV cache token count exceeds the int32 slot index limit")
-        self._storage = KVStorage(self.n_tokens, n_layers, n_kv_heads, head_dim, self.device, dtype)
+        self._storage = KVStorage(self.n_tokens, n_layers, n_kv_heads, head_dim, self.device, dtype, four_bit=kv_dtype == "int4")
         self._req_pool = ReqToTokenPool(max_batch_size, max_seq_len, self.device)
         if self.contiguous:
             rows = torch.arange(max_batch_size * max_seq_len, dtype=torch.int32).view(max_batch_size, max_seq_len)
@@ -64,17 +76,21 @@ class PagePool:
 
     @classmethod
     def for_model(cls, config, max_batch_size: int, max_seq_len: int, device, dtype, page_size: int = DEFAULT_PAGE_SIZE,
-                  n_tokens: Optional[int] = None, paged: bool = True) -> "PagePool":
+                  n_tokens: Optional[int] = None, paged: bool = True, kv_dtype: str = "auto") -> "PagePool":
         """Pool sized for a model config; paged with a radix prefix index unless ``paged=False``."""
         head_dim = config.hidden_size // config.num_attention_heads
         if paged and n_tokens is None:
             n_tokens = max_batch_size * (-(-max_seq_len // page_size)) * page_size
         return cls(config.num_hidden_layers, config.num_key_value_heads, head_dim, max_batch_size, max_seq_len, device,
-                   dtype, page_size=page_size if paged else 1, n_tokens=n_tokens if paged else None)
+                   dtype, page_size=page_size if paged else 1, n_tokens=n_tokens if paged else None, kv_dtype=kv_dtype)
 
     strategy = property(lambda self: self._strategy)
     req_pool = property(lambda self: self._req_pool)
     storage = property(lambda self: self._storage)
+
+    def copy_pages(self, src: List[int], dst: List[int]):
+        """Copy pages in every layer (contiguous layout: whole rows), on the current stream."""
+        copy_pages_(self._storage.pools(), src, dst, self.max_seq_len if self.contiguous else self.page_size)
 
     def bind_tasks(self, req_indices: List[int], seq_lens: List[int], workspace: InferenceWorkspace, device=None,
                    start_pos: Optional[int] = None, incremental: bool = False,
@@ -107,12 +123,14 @@ class PagePool:
                 ti += list(range(n))
             tile_b, tile_i = ws.put_int(ws.q_tile_to_batch, tb), ws.put_int(ws.q_tile_to_index, ti)
             gather = None
-            in_place = not self.contiguous and self.page_size in (8, 16, 32, 64)  # the prefill kernel walks the table itself
+            # the prefill kernel walks the table itself; rows of a 4-bit pool are read back into packed tensors first
+            in_place = not self.contiguous and self.page_size in (8, 16, 32, 64) and self.kv_dtype != "int4"
             if self.device.type == "cuda" and not in_place:  # one index for "all keys of the batch": gathered once per layer
                 gather = torch.cat([host[r, :n] for r, n in zip(req_indices, seq_lens)]).to(torch.int64).to(self.device, non_blocking=True)
             return KVCache(self._storage.k_buffer, self._storage.v_buffer, self._req_pool.req_to_token, rows, lens_t,
                            out_cache_loc, max(seq_lens), kv_indptr, qo, tile_b, tile_i, q_lens=q_lens, kv_lens=list(seq_lens),
-                           kv_gather_loc=gather, page_size=1 if self.contiguous else self.page_size)
+                           kv_gather_loc=gather, page_size=1 if self.contiguous else self.page_size,
+                           k_meta=self._storage.k_meta, v_meta=self._storage.v_meta)
         # slot of every request's newest position: one gather over the host table (a Python loop over the requests costs
         # more than the rest of the step's bookkeeping at large batch sizes)
         loc = host[torch.as_tensor(req_indices, dtype=torch.long), torch.as_tensor(seq_lens, dtype=torch.long) - 1]
@@ -126,7 +144,7 @@ class PagePool:
         return KVCache(self._storage.k_buffer, self._storage.v_buffer, self._req_pool.req_to_token, rows, lens_t,
                        out_cache_loc, max_len, kv_indptr, ws.qo_indptr[: b + 1], None, None, ws.decode_o_part,
                        ws.decode_ml_part, ws.decode_out, ws.decode_counters, q_lens=[1] * b, kv_lens=list(seq_lens),
-                       decode_splits=splits)
+                       decode_splits=splits, k_meta=self._storage.k_meta, v_meta=self._storage.v_meta)
 
 
 class TaskCacheManager:
@@ -151,6 +169,32 @@ class TaskCacheManager:
             return False
         self._strategy.write_indices(state, prompt_ids)
         state.length = len(prompt_ids)
+        return True
+
+    def task_fork(self, task_id: str, new_task_id: str, length: Optional[int] = None) -> bool:
+        """Start ``new_task_id`` as a continuation of the first ``length`` cached positions of ``task_id`` (default: all of
+        them).  Pages that lie wholly inside are shared, the one that is shared in part is copied (one launch for every
+        layer), so each of the two may go on by itself.  False when no request row or page is left.  The positions must have
+        been computed: a position that was only reserved (``task_extend``) is not yet in the cache."""
+        src = self._states.get(task_id)
+        if src is None:
+            raise KeyError(f"unknown task {task_id!r}")
+        if new_task_id in self._states:
+            raise ValueError(f"task {new_task_id!r} already exists")
+        length = src.length if length is None else length
+        if not 0 <= length <= src.length:
+            raise ValueError(f"length must be in [0, {src.length}], got {length}")
+        self._bind_state = None
+        rows = self._req_pool.alloc(1)
+        if rows is None:
+            return False
+        state = TaskCacheState(req_idx=rows[0], length=length, cached=length)
+        if not self._strategy.fork(src, state, length, self._pool.copy_pages):
+            self._strategy.free(state)
+            self._req_pool.free([state.req_idx])
+            return False
+        self._strategy.write_indices(state, [])
+        self._states[new_task_id] = state
         return True
 
     def task_free(self, task_id: str):

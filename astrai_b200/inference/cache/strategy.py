@@ -266,6 +266,11 @@ class AllocationStrategy:
     def extend(self, state: TaskCacheState, pos: int) -> bool:
         raise NotImplementedError
 
+    def fork(self, src: TaskCacheState, dst: TaskCacheState, length: int, copy: Callable[[List[int], List[int]], None]) -> bool:
+        """Give ``dst`` the first ``length`` positions of ``src``; ``copy(sources, destinations)`` copies what they cannot
+        share.  False when there is no room."""
+        raise NotImplementedError
+
     def write_indices(self, state: TaskCacheState, prompt_ids: List[int]) -> None:
         raise NotImplementedError
 
@@ -283,6 +288,10 @@ class ContiguousStrategy(AllocationStrategy):
         pass
 
     def extend(self, state, pos):
+        return True
+
+    def fork(self, src, dst, length, copy):
+        copy([src.req_idx], [dst.req_idx])  # a row of the contiguous layout is one page
         return True
 
     def write_indices(self, state, prompt_ids):
@@ -333,6 +342,19 @@ class PagedStrategy(AllocationStrategy):
             begin = page * self._page_size
             room = min(self._page_size, self._req_pool.max_context_len - begin)
             self._req_pool.write_row(state.req_idx, begin, self._slots([p])[:room])  # the whole page in one copy
+        return True
+
+    def fork(self, src, dst, length, copy):
+        whole, part = divmod(length, self._page_size)
+        for p in src.pages[:whole]:
+            self._alloc.inc_ref(p)
+        dst.pages = list(src.pages[:whole])
+        if part:  # the page behind the whole ones will be written by both: dst gets its own
+            p = self._alloc.alloc()
+            if p < 0:
+                return False
+            dst.pages.append(p)
+            copy([src.pages[whole]], [p])
         return True
 
     def write_indices(self, state, prompt_ids):

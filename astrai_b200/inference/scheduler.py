@@ -30,10 +30,12 @@ class InferenceScheduler:
                  dtype=None, cache: Optional[PagePool] = None, enable_cuda_graph: bool = True, backend=None,
                  page_size: int = 16, kv_cache_tokens: Optional[int] = None, paged: bool = True,
                  max_prefill_tokens: int = 8192, chunked_prefill: bool = False, prefill_defer_steps: int = 8,
-                 prefill_defer_min_batch: int = 32, prefill_defer_tokens: int = 2048, tp_group=None, tp_size: int = 1):
+                 prefill_defer_min_batch: int = 32, prefill_defer_tokens: int = 2048, tp_group=None, tp_size: int = 1,
+                 kv_dtype: str = "auto"):
         """``tp_size > 1`` (or a ``tp_group``): tensor-parallel serving - the model is cut over the ranks of the group,
         every rank runs this scheduler in lockstep and the first rank alone talks to clients
-        (:mod:`astrai_b200.parallel.tp_inference`; the other ranks call :meth:`follow`)."""
+        (:mod:`astrai_b200.parallel.tp_inference`; the other ranks call :meth:`follow`).  ``kv_dtype="int4"`` holds the
+        cache in 4 bits (:mod:`astrai_b200.ops.kv4`): 3.2 times as many tokens in the same memory; ``"auto"``: in ``dtype``."""
         self._control = None
         if tp_group is not None or tp_size > 1:
             from astrai_b200.parallel.tp_inference import ReplicatedControl, shard_for_inference_
@@ -51,7 +53,8 @@ class InferenceScheduler:
         self.device = torch.device(device) if device is not None else p.device
         self.dtype = dtype or p.dtype
         self._cache = cache if cache is not None else PagePool.for_model(
-            cfg, max_batch_size, max_seq_len, self.device, self.dtype, page_size=page_size, n_tokens=kv_cache_tokens, paged=paged)
+            cfg, max_batch_size, max_seq_len, self.device, self.dtype, page_size=page_size, n_tokens=kv_cache_tokens, paged=paged,
+            kv_dtype=kv_dtype)
         self._metrics = MetricsCollector()
         self._task_cache = TaskCacheManager(self._cache)
         self._task_mgr = TaskManager(tokenizer, max_batch_size, max_seq_len, metrics=self._metrics)
@@ -360,37 +363,71 @@ class InferenceScheduler:
     # -- synchronous path (RL rollout) -------------------------------------------------------------------------------------------
     def run_batch(self, prompt_ids_list: List[List[int]], *, max_tokens: Optional[int] = None, temperature: float = 1.0,
                   top_p: float = 1.0, top_k: int = 50, frequency_penalty: float = 0.0, rep_window: int = 64,
-                  return_logprobs: bool = False):
-        """Generate for already tokenised prompts on the calling thread; prompts that do not fit yield empty results."""
+                  return_logprobs: bool = False, samples_per_prompt: int = 1):
+        """Generate for already tokenised prompts on the calling thread; prompts that do not fit yield empty results.
+
+        ``samples_per_prompt`` answers are drawn for every prompt (results prompt after prompt).  The prompt is prefilled
+        once and its cache forked for the other answers, which compute the prompt's last position only."""
+        if samples_per_prompt < 1:
+            raise ValueError(f"samples_per_prompt must be at least 1, got {samples_per_prompt}")
         stop_ids = set(self._task_mgr.tokenizer.stop_ids)
         tasks: List[Optional[Task]] = []
+
+        def name() -> str:
+            self._batch_serial += 1  # ids must sort alike on every rank of a tensor-parallel replica: a counter, not a random id
+            return f"batch_{self._batch_serial:012d}" if self._control is not None else f"batch_{uuid.uuid4().hex[:8]}"
+
         for ids in prompt_ids_list:
             room = self.max_seq_len - len(ids)
             budget = room if max_tokens is None else min(max_tokens, room)
             if len(ids) >= self.max_seq_len or budget <= 0:
                 tasks.append(None)
                 continue
-            self._batch_serial += 1  # ids must sort alike on every rank of a tensor-parallel replica: a counter, not a random id
-            name = f"batch_{self._batch_serial:012d}" if self._control is not None else f"batch_{uuid.uuid4().hex[:8]}"
-            task = Task(name, list(ids), budget, temperature, top_p, top_k, frequency_penalty, rep_window)
+            task = Task(name(), list(ids), budget, temperature, top_p, top_k, frequency_penalty, rep_window)
             if not self._task_cache.task_alloc(task.task_id, task.prompt_ids):
                 tasks.append(None)
                 continue
             task.input_tokens = len(task.prompt_ids)
             self._metrics.register(task.task_id)
             tasks.append(task)
+        leaders = tasks
+        if samples_per_prompt > 1:  # slot 0 of a prompt's answers is its leader's, the others are filled by forks of it
+            tasks = [t if i == 0 else None for t in leaders for i in range(samples_per_prompt)]
+        unforked = {id(t): k * samples_per_prompt for k, t in enumerate(leaders) if t is not None and samples_per_prompt > 1}
+
+        def fork_ready() -> List[Task]:
+            forks = []
+            for k, t in enumerate(leaders):
+                if t is None or not t.prefill_done or unforked.pop(id(t), None) is None:
+                    continue
+                for i in range(1, samples_per_prompt):
+                    twin = Task(name(), list(t.prompt_ids), t.max_tokens, temperature, top_p, top_k, frequency_penalty, rep_window)
+                    # all but the last position: that one is computed again for the logits, in a page of the twin's own
+                    if not self._task_cache.task_fork(t.task_id, twin.task_id, len(t.prompt_ids) - 1):
+                        break
+                    if not self._task_cache.task_extend(twin.task_id, len(t.prompt_ids) - 1):
+                        self._task_cache.task_free(twin.task_id)
+                        break
+                    twin.input_tokens = len(twin.prompt_ids)
+                    self._metrics.register(twin.task_id)
+                    tasks[k * samples_per_prompt + i] = twin
+                    forks.append(twin)
+            return forks
+
         try:
             live = [t for t in tasks if t is not None]
             while live:
                 before = sum(t.prefill_pos or 0 for t in live)
                 decoded, _ = self._step(live, return_logprobs=return_logprobs)
                 produced = {id(t) for t in decoded}
-                # a request without a token this step stays only while its (chunked) prefill is still advancing
-                waiting = [t for t in live if id(t) not in produced and self.chunked_prefill and not t.prefill_done
-                           and t.status != TaskStatus.ABORTED]
+                # a request without a token this step stays only while its (chunked) prefill is still advancing, or, a fork,
+                # while its one-token prefill is put off behind a large decode batch
+                waiting = [t for t in live if id(t) not in produced and (self.chunked_prefill or samples_per_prompt > 1)
+                           and not t.prefill_done and t.status != TaskStatus.ABORTED]
                 if not decoded and sum(t.prefill_pos or 0 for t in waiting) == before:
                     waiting = []
-                live = [t for t in live if (id(t) in produced and not t.is_finished(stop_ids)) or t in waiting]
+                forks = fork_ready() if unforked else []
+                live = [t for t in live if (id(t) in produced and not t.is_finished(stop_ids)) or t in waiting] + forks
         finally:
             for t in tasks:
                 if t is not None:

@@ -58,7 +58,10 @@ def messages_from_fields(instruction: str = "", user_input: str = "", output: st
 
 class RolloutGenerator:
     def __init__(self, scheduler, tokenizer, max_tokens: int = 1024, group_size: int = 8, temperature: float = 1.0,
-                 top_k: int = 0, top_p: float = 1.0, frequency_penalty: float = 0.0, rep_window: int = 64):
+                 top_k: int = 0, top_p: float = 1.0, frequency_penalty: float = 0.0, rep_window: int = 64,
+                 share_prompts: bool = False):
+        """``share_prompts``: prefill each prompt once and fork its cache for the group's other responses."""
+        self.share_prompts = bool(share_prompts)
         self.scheduler, self.tokenizer = scheduler, tokenizer
         self.max_tokens, self.group_size = max_tokens, group_size
         self.sampling = dict(temperature=temperature, top_k=top_k, top_p=top_p, frequency_penalty=frequency_penalty,
@@ -114,8 +117,12 @@ class RolloutGenerator:
     def _generate(self, batch) -> RawRollout:
         texts, prompt_ids = self._render(self._conversations(batch))
         b, g = len(texts), self.group_size
-        requests = [list(ids) for ids in prompt_ids for _ in range(g)]
-        results = self.scheduler.run_batch(requests, max_tokens=self.max_tokens, return_logprobs=True, **self.sampling)
+        if self.share_prompts:
+            results = self.scheduler.run_batch([list(ids) for ids in prompt_ids], max_tokens=self.max_tokens, return_logprobs=True,
+                                               samples_per_prompt=g, **self.sampling)
+        else:
+            requests = [list(ids) for ids in prompt_ids for _ in range(g)]
+            results = self.scheduler.run_batch(requests, max_tokens=self.max_tokens, return_logprobs=True, **self.sampling)
         if len(results) != b * g:
             raise RuntimeError(f"the scheduler returned {len(results)} generations for {b * g} requests")
         if any(len(toks) != len(lps) for toks, lps in results):
