@@ -379,8 +379,11 @@ Kv4Pools kv4_check(const char* what, const Tensor& k_codes, const Tensor& k_meta
     TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 4 && t->size(0) == p.slots && t->size(1) == p.heads &&
                     t->size(2) == p.dim / 32 && t->size(3) == 2,
                 what, ": k_meta / v_meta must be bf16 [slots, heads, head_dim / 32, 2]");
-  for (const Tensor* t : {&k_codes, &k_meta, &v_codes, &v_meta})
-    TORCH_CHECK((reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0, what, ": the pools must be 16-byte aligned");
+  const uintptr_t word = p.dim == 32 ? 4 : p.dim == 64 ? 8 : 16;  // a row's middles and steps, read in pieces of 16 bytes at most
+  for (const Tensor* t : {&k_codes, &v_codes})
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, what, ": the codes must be 16-byte aligned");
+  for (const Tensor* t : {&k_meta, &v_meta})
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % word == 0, what, ": k_meta / v_meta must be ", (int)word, "-byte aligned");
   return p;
 }
 
@@ -428,11 +431,11 @@ std::tuple<Tensor, Tensor> kv4_gather(const Tensor& k_codes, const Tensor& k_met
   return {k, v};
 }
 
-// Decode attention over the 4-bit pools; see kv4_decode in launchers.h.  splits = 0: chosen from max_len.  Scratch: all
-// three tensors or none (allocated for the call).
+// Decode attention over the 4-bit pools; see kv4_decode in launchers.h.  Scratch: all three tensors or none (allocated
+// for the call).
 void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_codes, Tensor& v_meta, const Tensor& req_to_token,
                  const Tensor& req_pool_indices, const Tensor& seq_lens, const std::optional<Tensor>& k_new, const std::optional<Tensor>& v_new,
-                 double scale, int64_t max_len, int64_t splits, const std::optional<Tensor>& o_part_, const std::optional<Tensor>& ml_part_,
+                 double scale, int64_t max_len, const std::optional<Tensor>& o_part_, const std::optional<Tensor>& ml_part_,
                  const std::optional<Tensor>& counters_, Tensor& out) {
   const Kv4Pools p = kv4_check("kv4_decode", k_codes, k_meta, v_codes, v_meta);
   const auto dev = k_codes.device();
@@ -455,23 +458,25 @@ void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_co
   const c10::cuda::CUDAGuard guard(dev);
   const int given = o_part_.has_value() + ml_part_.has_value() + counters_.has_value();
   TORCH_CHECK(given == 0 || given == 3, "kv4_decode: the workspace is three tensors (o_part, ml_part, counters)");
-  constexpr int64_t kMaxSplits = 32;
-  const int64_t limit = given ? o_part_->dim() == 4 ? o_part_->size(2) : 0 : kMaxSplits;
-  if (splits <= 0) splits = ab::kv4_decode_splits((int)B, (int)Hkv, max_len > 0 ? max_len : req_to_token.size(1), (int)limit);
-  TORCH_CHECK(limit >= 1 && splits <= limit, "kv4_decode: ", splits, " splits, the workspace holds ", limit);
+  auto aligned = [](const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; };
+  TORCH_CHECK(aligned(out), "kv4_decode: out must start on a 16-byte boundary");
   Tensor o_part, ml_part, counters;
+  int64_t parts;
   if (given) {
     o_part = *o_part_, ml_part = *ml_part_, counters = *counters_;
+    parts = o_part.dim() == 4 ? o_part.size(2) : 0;
     auto fits = [&](const Tensor& t, int64_t last) {
       return t.device() == dev && t.is_contiguous() && t.scalar_type() == at::kFloat && t.dim() == 4 && t.size(0) >= B && t.size(1) == Hq &&
-             t.size(2) == limit && t.size(3) == last;
+             t.size(2) == parts && t.size(3) == last && aligned(t);
     };
-    TORCH_CHECK(fits(o_part, D) && fits(ml_part, 2), "kv4_decode: workspace o_part / ml_part must be fp32 [>= batch, heads, splits, head_dim / 2 numbers]");
+    TORCH_CHECK(parts >= 1 && fits(o_part, D) && fits(ml_part, 2),
+                "kv4_decode: workspace o_part / ml_part must be fp32 [>= batch, heads, parts, head_dim / 2 numbers], 16-byte aligned");
     TORCH_CHECK(counters.device() == dev && counters.is_contiguous() && counters.scalar_type() == at::kInt && counters.numel() >= B * Hkv,
                 "kv4_decode: workspace counters must be int32 [>= batch * kv_heads], zero before the first call");
   } else {
+    parts = B == 0 ? 1 : std::min<int64_t>(32, 444 / (B * Hkv) + 2);  // room for a whole wave, 32 at most
     const auto f32 = q_.options().dtype(at::kFloat);
-    o_part = at::empty({B, Hq, splits, D}, f32), ml_part = at::empty({B, Hq, splits, 2}, f32);
+    o_part = at::empty({B, Hq, parts, D}, f32), ml_part = at::empty({B, Hq, parts, 2}, f32);
     counters = at::zeros({B * Hkv}, q_.options().dtype(at::kInt));
   }
   const Tensor q = q_.is_contiguous() && (reinterpret_cast<uintptr_t>(q_.data_ptr()) & 15) == 0 ? q_ : q_.clone(at::MemoryFormat::Contiguous);
@@ -485,8 +490,8 @@ void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_co
                                 req_to_token.data_ptr<int>(), req_pool_indices.data_ptr<int>(), (const long long*)seq_lens.data_ptr<int64_t>(),
                                 k_new ? kn.data_ptr() : nullptr, v_new ? vn.data_ptr() : nullptr, o_part.data_ptr<float>(),
                                 ml_part.data_ptr<float>(), counters.data_ptr<int>(), out.data_ptr(), (int)B, (int)Hq, (int)Hkv, (int)D,
-                                (int)req_to_token.size(1), (int)req_to_token.size(0), p.slots, (float)scale, (int)splits,
-                                (int)o_part.size(2), stream());
+                                (int)req_to_token.size(1), (int)req_to_token.size(0), p.slots, (float)scale, (int)parts,
+                                max_len, stream());
   TORCH_CHECK(rc == 0, "kv4_decode launch failed with code ", rc);
 }
 
@@ -1275,7 +1280,7 @@ TORCH_LIBRARY(astrai_b200, m) {
   m.def("flash_fwd(Tensor q, Tensor k, Tensor v, Tensor? cu_q, Tensor? cu_k, int batch, int sq, int sk, int max_q, bool causal, float scale) -> (Tensor, Tensor)", &flash_fwd);
   m.def("kv4_append_(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor loc) -> ()", &kv4_append_);
   m.def("kv4_gather(Tensor k_codes, Tensor k_meta, Tensor v_codes, Tensor v_meta, Tensor loc) -> (Tensor, Tensor)", &kv4_gather);
-  m.def("kv4_decode_(Tensor q, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor req_to_token, Tensor req_pool_indices, Tensor seq_lens, Tensor? k_new, Tensor? v_new, float scale, int max_len, int splits, Tensor? o_part, Tensor? ml_part, Tensor? counters, Tensor(e!) out) -> ()", &kv4_decode_);
+  m.def("kv4_decode_(Tensor q, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor req_to_token, Tensor req_pool_indices, Tensor seq_lens, Tensor? k_new, Tensor? v_new, float scale, int max_len, Tensor? o_part, Tensor? ml_part, Tensor? counters, Tensor(e!) out) -> ()", &kv4_decode_);
   m.def("copy_pages_(Tensor(a!)[] pools, int[] src, int[] dst, int page_size) -> ()", &copy_pages_);
   m.def("flash_fwd_paged(Tensor q, Tensor k_pool, Tensor v_pool, Tensor cu_q, Tensor cu_k, Tensor table, Tensor rows, int page, int max_q, bool causal, float scale) -> Tensor", &flash_fwd_paged);
   m.def("flash_bwd(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, Tensor? cu_q, Tensor? cu_k, int batch, int sq, int sk, int max_q, int max_k, bool causal, float scale) -> (Tensor, Tensor, Tensor)", &flash_bwd);

@@ -279,13 +279,14 @@ int kv4_append(const void* k, const void* v, void* k_codes, void* k_meta, void* 
 // k / v out: bf16 [tokens, heads, D] contiguous.
 int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, const void* loc, bool loc64, void* k,
                void* v, long long tokens, int heads, int head_dim, long long n_slots, cudaStream_t st);
-int kv4_decode_splits(int batch, int n_kv_heads, long long max_len, int max_splits);
-// Scratch as for paged_decode.  k_new / v_new (both or neither): bf16 [batch, n_kv_heads, D], stored into the slot of the
-// last position first.  Returns also -1: more than 8 query heads per kv head, -2: splits.
-int kv4_decode(const void* q, const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, const int* req_to_token,
-               const int* req_pool_indices, const long long* seq_lens, const void* k_new, const void* v_new, float* o_part, float* ml_part,
-               int* counters, void* out, int batch, int n_q_heads, int n_kv_heads, int head_dim, int max_ctx, int table_rows,
-               long long n_slots, float scale, int splits, int max_splits, cudaStream_t st);
+// Decode attention.  Scratch: o_part fp32 [batch, n_q_heads, parts, D] and ml_part [batch, n_q_heads, parts, 2], 16-byte
+// aligned, used as flat arrays; counters int32 [batch * n_kv_heads], zero before the first call.  max_len sizes the grid
+// (0: the table's width); longer requests are served all the same.  k_new / v_new (both or neither): bf16 [batch, n_kv_heads, D],
+// stored into the slot of the last position first.  Returns also -1: more than 8 query heads per kv head, -2: parts.
+int kv4_decode(const void* q, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const int* req_to_token, const int* req_pool_indices,
+               const long long* seq_lens, const void* k_new, const void* v_new, float* o_part, float* ml_part, int* counters, void* out,
+               int batch, int n_q_heads, int n_kv_heads, int head_dim, int max_ctx, int table_rows, long long n_slots, float scale, int parts,
+               long long max_len, cudaStream_t st);
 
 // Page copies of one launch: page dst[i] = page src[i] in every layer of every pool (kv4.cu).  No destination may be a
 // source or occur twice.

@@ -26,7 +26,6 @@ from astrai_b200.ops import native
 
 HEAD_DIMS = (32, 64, 128, 256)
 GROUP = 32
-MAX_SPLITS = 32
 
 
 def _ops():
@@ -116,17 +115,18 @@ def kv4_gather(k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_meta: Tensor,
     return tuple(torch.where(ok[:, None, None], x, torch.zeros_like(x)).to(torch.bfloat16) for x in (k, v))
 
 
-def kv4_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device, splits: int = MAX_SPLITS):
-    """Scratch of :func:`kv4_decode` for up to ``batch`` requests: ``(o_part, ml_part, counters)``.  Calls that may run at the
+def kv4_decode_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device, parts: int = 32):
+    """Scratch of :func:`kv4_decode` for up to ``batch`` requests: ``(o_part, ml_part, counters)``, with room for ``parts``
+    partial results per request on average (fewer than 32 can leave a part of the GPU idle when there are few requests).  Calls that may run at the
     same time (two streams, two captured graphs replayed side by side) need a workspace each."""
-    return (torch.empty((batch, n_q_heads, splits, head_dim), dtype=torch.float32, device=device),
-            torch.empty((batch, n_q_heads, splits, 2), dtype=torch.float32, device=device),
+    return (torch.empty((batch, n_q_heads, parts, head_dim), dtype=torch.float32, device=device),
+            torch.empty((batch, n_q_heads, parts, 2), dtype=torch.float32, device=device),
             torch.zeros(batch * n_kv_heads, dtype=torch.int32, device=device))
 
 
 def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_meta: Tensor, req_to_token: Tensor,
                req_pool_indices: Tensor, seq_lens: Tensor, k_new: Optional[Tensor] = None, v_new: Optional[Tensor] = None, *,
-               scale: Optional[float] = None, max_len: int = 0, splits: int = 0, workspace=None, out: Optional[Tensor] = None) -> Tensor:
+               scale: Optional[float] = None, max_len: int = 0, workspace=None, out: Optional[Tensor] = None) -> Tensor:
     """Attention of one query per request over its rows of the 4-bit pools.
 
     ``q [batch, heads, D]``; request ``i`` has ``seq_lens[i]`` positions (int64) whose slots are
@@ -135,16 +135,16 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
     positions whose slot is outside the pool are left out.  The numbers of the cache enter unrounded, sums and softmax are
     fp32, the result is bf16.
 
-    ``max_len`` (the longest length, when the host knows it) and ``splits`` decide into how many parts the keys of a
-    request are cut; 0 lets the table's width and the batch decide.  ``workspace``: see :func:`kv4_decode_workspace`; without
-    one the call allocates its own scratch."""
+    The keys of the whole batch are spread evenly over the GPU, whatever the lengths.  ``max_len``: the longest length, when
+    the host knows it (0: the table's width) - it sizes the launch, a longer request is served all the same.  ``workspace``:
+    see :func:`kv4_decode_workspace`; without one the call allocates its own scratch."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     if k_codes.is_cuda:
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         o_part, ml_part, counters = workspace if workspace is not None else (None, None, None)
         _ops().kv4_decode_(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new, scale,
-                           max_len, splits, o_part, ml_part, counters, out)
+                           max_len, o_part, ml_part, counters, out)
         return out
     b, hq, d = q.shape
     hkv, slots = k_codes.shape[1], k_codes.shape[0]

@@ -162,8 +162,9 @@ def test_decode_attention(lens, heads, kv_heads, dim):
 
     pools, table, rows, n, q, new = _case(lens, heads, kv_heads, dim, seed=heads + dim)
     scale = dim ** -0.5
-    for splits in (0, 1, 3):
-        _near(ops.kv4_decode(q, *pools, table, rows, n, splits=splits), _expected(pools, table, rows, n, q, scale))
+    for parts in (None, 1, 2, 32):  # one part: a single CTA walks every request
+        work = parts and ops.kv4_decode_workspace(len(lens), heads, kv_heads, dim, "cuda", parts=parts)
+        _near(ops.kv4_decode(q, *pools, table, rows, n, workspace=work), _expected(pools, table, rows, n, q, scale))
     # with the step's own rows: stored first, then attended to
     stored = [t.clone() for t in pools]
     live = n > 0
@@ -285,9 +286,9 @@ def test_decode_refusals():
     wrong = [dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.repeat(1, 5, 1)), dict(seq_lens=n.int()), dict(seq_lens=n[:1]),
              dict(req_pool_indices=rows.long()), dict(req_to_token=table.long()), dict(req_to_token=table.t()), dict(k_codes=pools[0][:, :1]),
              dict(k_meta=pools[1].float()), dict(v_codes=pools[2].cpu()), dict(k_new=new[0]), dict(k_new=new[0].float(), v_new=new[1]),
-             dict(k_new=new[0][:1], v_new=new[1][:1]), dict(splits=33), dict(out=q.float()), dict(out=q[:1]),
+             dict(k_new=new[0][:1], v_new=new[1][:1]), dict(out=q.float()), dict(out=q[:1]),
              dict(workspace=ops.kv4_decode_workspace(1, 4, 2, 64, "cuda")), dict(workspace=ops.kv4_decode_workspace(2, 4, 2, 128, "cuda")),
-             dict(req_to_token=table[:0])]
+             dict(req_to_token=table[:0]), dict(out=torch.empty(q.numel() + 1, device="cuda", dtype=torch.bfloat16)[1:].view(q.shape))]
     for bad in wrong:
         with pytest.raises(RuntimeError, match="kv4_decode"):
             ops.kv4_decode(**{**ok, **bad})
