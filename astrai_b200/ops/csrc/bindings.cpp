@@ -469,12 +469,12 @@ void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_co
       return t.device() == dev && t.is_contiguous() && t.scalar_type() == at::kFloat && t.dim() == 4 && t.size(0) >= B && t.size(1) == Hq &&
              t.size(2) == parts && t.size(3) == last && aligned(t);
     };
-    TORCH_CHECK(parts >= 1 && fits(o_part, D) && fits(ml_part, 2),
-                "kv4_decode: workspace o_part / ml_part must be fp32 [>= batch, heads, parts, head_dim / 2 numbers], 16-byte aligned");
+    TORCH_CHECK(parts >= 2 && fits(o_part, D) && fits(ml_part, 2),
+                "kv4_decode: workspace o_part / ml_part must be fp32 [>= batch, heads, >= 2 parts, head_dim / 2 numbers], 16-byte aligned");
     TORCH_CHECK(counters.device() == dev && counters.is_contiguous() && counters.scalar_type() == at::kInt && counters.numel() >= B * Hkv,
                 "kv4_decode: workspace counters must be int32 [>= batch * kv_heads], zero before the first call");
   } else {
-    parts = B == 0 ? 1 : std::min<int64_t>(32, 444 / (B * Hkv) + 2);  // room for a whole wave, 32 at most
+    parts = B == 0 ? 1 : std::min<int64_t>(32, 148 / (B * Hkv) + 3);  // room for a whole wave, 32 at most
     const auto f32 = q_.options().dtype(at::kFloat);
     o_part = at::empty({B, Hq, parts, D}, f32), ml_part = at::empty({B, Hq, parts, 2}, f32);
     counters = at::zeros({B * Hkv}, q_.options().dtype(at::kInt));

@@ -162,7 +162,7 @@ def test_decode_attention(lens, heads, kv_heads, dim):
 
     pools, table, rows, n, q, new = _case(lens, heads, kv_heads, dim, seed=heads + dim)
     scale = dim ** -0.5
-    for parts in (None, 1, 2, 32):  # one part: a single CTA walks every request
+    for parts in (None, 2, 3, 32):  # two parts: a single CTA walks every request
         work = parts and ops.kv4_decode_workspace(len(lens), heads, kv_heads, dim, "cuda", parts=parts)
         _near(ops.kv4_decode(q, *pools, table, rows, n, workspace=work), _expected(pools, table, rows, n, q, scale))
     # with the step's own rows: stored first, then attended to
@@ -287,7 +287,7 @@ def test_decode_refusals():
              dict(req_pool_indices=rows.long()), dict(req_to_token=table.long()), dict(req_to_token=table.t()), dict(k_codes=pools[0][:, :1]),
              dict(k_meta=pools[1].float()), dict(v_codes=pools[2].cpu()), dict(k_new=new[0]), dict(k_new=new[0].float(), v_new=new[1]),
              dict(k_new=new[0][:1], v_new=new[1][:1]), dict(out=q.float()), dict(out=q[:1]),
-             dict(workspace=ops.kv4_decode_workspace(1, 4, 2, 64, "cuda")), dict(workspace=ops.kv4_decode_workspace(2, 4, 2, 128, "cuda")),
+             dict(workspace=ops.kv4_decode_workspace(1, 4, 2, 64, "cuda")), dict(workspace=ops.kv4_decode_workspace(2, 4, 2, 64, "cuda", parts=1)), dict(workspace=ops.kv4_decode_workspace(2, 4, 2, 128, "cuda")),
              dict(req_to_token=table[:0]), dict(out=torch.empty(q.numel() + 1, device="cuda", dtype=torch.bfloat16)[1:].view(q.shape))]
     for bad in wrong:
         with pytest.raises(RuntimeError, match="kv4_decode"):
