@@ -10,111 +10,118 @@
 namespace ab {
 
 // ------------------------------------------------------------------------------------------------------- store rows
-// D / 8 lanes a row, blockIdx.y = 0 for keys, 1 for values.  A slot outside the pool is skipped.
+// D / 8 lanes a row, a key row and a value row each.  A slot outside the pool is skipped.
 template <int D, typename Loc>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v,
                                                          uint8_t* __restrict__ k_codes, uint32_t* __restrict__ k_meta,
                                                          uint8_t* __restrict__ v_codes, uint32_t* __restrict__ v_meta,
-                                                         const Loc* __restrict__ loc, long long rows, int heads, long long n_slots,
+                                                         const Loc* __restrict__ loc, int rows, int heads, long long n_slots,
                                                          long long k_tok, long long k_head, long long v_tok, long long v_head) {
   constexpr int LPR = D / 8;
-  const bool key = blockIdx.y == 0;
   const int l = threadIdx.x % LPR;
-  const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / LPR;
-  const long long t = r / heads;
-  const int h = (int)(r - t * heads);
+  const int r = (blockIdx.x * 256 + threadIdx.x) / LPR, t = r / heads, h = r - t * heads;
   const long long slot = r < rows ? (long long)loc[t] : -1;
   const bool live = slot >= 0 && slot < n_slots;
   const long long at = live ? slot * heads + h : 0;
-  const __nv_bfloat16* src = key ? k + t * k_tok + h * k_head : v + t * v_tok + h * v_head;
-  kv4_store_row<D>(live, key, l, src, (key ? k_codes : v_codes) + at * (D / 2), (key ? k_meta : v_meta) + at * (D / 32));
-}
-
-int kv4_append(const void* k, const void* v, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* loc, bool loc64,
-               long long tokens, int heads, int head_dim, long long n_slots, long long k_tok, long long k_head, long long v_tok,
-               long long v_head, cudaStream_t st) {
-  const long long rows = tokens * heads;
-  if (rows == 0) return 0;
-  const long long blocks = (rows * (head_dim / 8) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -4;
-  const dim3 grid((unsigned)blocks, 2);
-#define AB_APPEND(DD, LL)                                                                                                     \
-  kv4_append_kernel<DD, LL><<<grid, 256, 0, st>>>((const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (uint8_t*)k_codes,         \
-                                                  (uint32_t*)k_meta, (uint8_t*)v_codes, (uint32_t*)v_meta, (const LL*)loc,     \
-                                                  rows, heads, n_slots, k_tok, k_head, v_tok, v_head)
-#define AB_APPEND_D(DD) \
-  if (loc64) AB_APPEND(DD, long long); else AB_APPEND(DD, int)
-  switch (head_dim) {
-    case 32: AB_APPEND_D(32); break;
-    case 64: AB_APPEND_D(64); break;
-    case 128: AB_APPEND_D(128); break;
-    case 256: AB_APPEND_D(256); break;
-    default: return -3;
-  }
-#undef AB_APPEND_D
-#undef AB_APPEND
-  return cudaGetLastError() == cudaSuccess ? 0 : -5;
+  kv4_store_row<D>(live, true, l, k + t * k_tok + h * k_head, k_codes + at * (D / 2), k_meta + at * (D / 32));
+  kv4_store_row<D>(live, false, l, v + t * v_tok + h * v_head, v_codes + at * (D / 2), v_meta + at * (D / 32));
 }
 
 // -------------------------------------------------------------------------------------------------------- read rows
 // The reverse, as bf16 rows [tokens, heads, D].  A slot outside the pool reads as zeros.
+__device__ __forceinline__ uint4 kv4_numbers(uint32_t word, uint32_t ms) {
+  const float m = __uint_as_float(ms << 16), s = __uint_as_float(ms & 0xffff0000u);
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)  // c in the low bits of 2^23 makes the number 2^23 + c
+    x[j] = fma_ieee(s, __uint_as_float(0x4b000000u | ((word >> (4 * j)) & 15u)) - 8388616.f, m);
+  Vec8<__nv_bfloat16> out;
+  out.pack(x);
+  return out.raw;
+}
+
 template <int D, typename Loc>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restrict__ k_codes, const uint32_t* __restrict__ k_meta,
                                                          const uint8_t* __restrict__ v_codes, const uint32_t* __restrict__ v_meta,
                                                          const Loc* __restrict__ loc, __nv_bfloat16* __restrict__ k,
-                                                         __nv_bfloat16* __restrict__ v, long long rows, int heads, long long n_slots) {
-  constexpr int LPR = D / 8;
-  const bool key = blockIdx.y == 0;
-  const int l = threadIdx.x % LPR;
-  const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / LPR;
-  if (r >= rows) return;
-  const long long t = r / heads;
-  const int h = (int)(r - t * heads);
-  const long long slot = (long long)loc[t];
-  Vec8<__nv_bfloat16> out;
-  out.raw = make_uint4(0, 0, 0, 0);
+                                                         __nv_bfloat16* __restrict__ v, int rows, int heads, long long n_slots) {
+  constexpr int LPR = D / 8, NG = D / 32;
+  const int l = threadIdx.x % LPR, g = l >> 2;
+  const int r = (blockIdx.x * 256 + threadIdx.x) / LPR, t = r / heads, h = r - t * heads;
+  const long long slot = r < rows ? (long long)loc[t] : -1;
+  uint32_t kw = 0x88888888u, vw = kw, kms = 0, vms = 0;
   if (slot >= 0 && slot < n_slots) {
     const long long at = slot * heads + h;
-    const uint8_t* codes = (key ? k_codes : v_codes) + at * (D / 2);
-    const uint32_t ms = (key ? k_meta : v_meta)[at * (D / 32) + (l >> 2)];
-    uint32_t word;
-    if (key) {
-      word = reinterpret_cast<const uint32_t*>(codes)[kv4_key_word<D>(l >> 2, l & 3)];
-    } else {
-      const uint16_t* halves = reinterpret_cast<const uint16_t*>(codes);
-      word = halves[kv4_value_half<D>(l >> 2, 2 * (l & 3))] | ((uint32_t)halves[kv4_value_half<D>(l >> 2, 2 * (l & 3) + 1)] << 16);
-    }
-    const float m = __uint_as_float(ms << 16), s = __uint_as_float(ms & 0xffff0000u);
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = fma_ieee(s, (float)((int)((word >> (4 * j)) & 15) - 8), m);
-    out.pack(x);
+    kw = reinterpret_cast<const uint32_t*>(k_codes + at * (D / 2))[kv4_key_word<D>(g, l & 3)];
+    vw = reinterpret_cast<const uint32_t*>(v_codes + at * (D / 2))[l];
+    kms = k_meta[at * NG + g], vms = v_meta[at * NG + g];
   }
-  out.store((key ? k : v) + r * D + 8 * l);
+  // numbers 8 l .. of a value row are the half words of group g, eighths 2 (l & 3) and the next: with two lanes
+  const int base = (threadIdx.x & 31) - l, h0 = kv4_value_half<D>(g, 2 * (l & 3)), h1 = kv4_value_half<D>(g, 2 * (l & 3) + 1);
+  const uint32_t w0 = __shfl_sync(0xffffffffu, vw, base + (h0 >> 1)), w1 = __shfl_sync(0xffffffffu, vw, base + (h1 >> 1));
+  vw = __byte_perm(w0, w1, (h0 & 1 ? 0x0032 : 0x0010) | (h1 & 1 ? 0x7600 : 0x5400));
+  if (r >= rows) return;
+  const long long to = (long long)r * D + 8 * l;
+  *reinterpret_cast<uint4*>(k + to) = kv4_numbers(kw, kms);
+  *reinterpret_cast<uint4*>(v + to) = kv4_numbers(vw, vms);
+}
+
+// Rows of one launch: their lanes are counted in 32 bits.
+constexpr long long kKv4Rows = 1 << 25;
+
+int kv4_append(const void* k, const void* v, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* loc, bool loc64,
+               long long tokens, int heads, int head_dim, long long n_slots, long long k_tok, long long k_head, long long v_tok,
+               long long v_head, cudaStream_t st) {
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return -3;
+  if (tokens == 0 || heads == 0) return 0;
+  if (heads > kKv4Rows) return -4;
+  const long long step = kKv4Rows / heads;
+  for (long long t = 0; t < tokens; t += step) {
+    const int rows = (int)((tokens - t < step ? tokens - t : step) * heads);
+    const int grid = ceil_div((long long)rows * (head_dim / 8), 256);
+#define AB_APPEND(DD, LL)                                                                                                       \
+  kv4_append_kernel<DD, LL><<<grid, 256, 0, st>>>((const __nv_bfloat16*)k + t * k_tok, (const __nv_bfloat16*)v + t * v_tok,      \
+                                                  (uint8_t*)k_codes, (uint32_t*)k_meta, (uint8_t*)v_codes, (uint32_t*)v_meta,    \
+                                                  (const LL*)loc + t, rows, heads, n_slots, k_tok, k_head, v_tok, v_head)
+#define AB_APPEND_D(DD) \
+  if (loc64) AB_APPEND(DD, long long); else AB_APPEND(DD, int)
+    switch (head_dim) {
+      case 32: AB_APPEND_D(32); break;
+      case 64: AB_APPEND_D(64); break;
+      case 128: AB_APPEND_D(128); break;
+      default: AB_APPEND_D(256); break;
+    }
+#undef AB_APPEND_D
+#undef AB_APPEND
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
 int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, const void* loc, bool loc64, void* k,
                void* v, long long tokens, int heads, int head_dim, long long n_slots, cudaStream_t st) {
-  const long long rows = tokens * heads;
-  if (rows == 0) return 0;
-  const long long blocks = (rows * (head_dim / 8) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -4;
-  const dim3 grid((unsigned)blocks, 2);
-#define AB_GATHER(DD, LL)                                                                                                       \
-  kv4_gather_kernel<DD, LL><<<grid, 256, 0, st>>>((const uint8_t*)k_codes, (const uint32_t*)k_meta, (const uint8_t*)v_codes,     \
-                                                  (const uint32_t*)v_meta, (const LL*)loc, (__nv_bfloat16*)k, (__nv_bfloat16*)v, \
-                                                  rows, heads, n_slots)
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return -3;
+  if (tokens == 0 || heads == 0) return 0;
+  if (heads > kKv4Rows) return -4;
+  const long long step = kKv4Rows / heads;
+  for (long long t = 0; t < tokens; t += step) {
+    const int rows = (int)((tokens - t < step ? tokens - t : step) * heads);
+    const int grid = ceil_div((long long)rows * (head_dim / 8), 256);
+    const long long to = t * heads * head_dim;
+#define AB_GATHER(DD, LL)                                                                                                          \
+  kv4_gather_kernel<DD, LL><<<grid, 256, 0, st>>>((const uint8_t*)k_codes, (const uint32_t*)k_meta, (const uint8_t*)v_codes,        \
+                                                  (const uint32_t*)v_meta, (const LL*)loc + t, (__nv_bfloat16*)k + to,              \
+                                                  (__nv_bfloat16*)v + to, rows, heads, n_slots)
 #define AB_GATHER_D(DD) \
   if (loc64) AB_GATHER(DD, long long); else AB_GATHER(DD, int)
-  switch (head_dim) {
-    case 32: AB_GATHER_D(32); break;
-    case 64: AB_GATHER_D(64); break;
-    case 128: AB_GATHER_D(128); break;
-    case 256: AB_GATHER_D(256); break;
-    default: return -3;
-  }
+    switch (head_dim) {
+      case 32: AB_GATHER_D(32); break;
+      case 64: AB_GATHER_D(64); break;
+      case 128: AB_GATHER_D(128); break;
+      default: AB_GATHER_D(256); break;
+    }
 #undef AB_GATHER_D
 #undef AB_GATHER
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
@@ -784,7 +791,16 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
   const Unit* src = reinterpret_cast<const Unit*>(base + c.src[pair] * page);
   Unit* dst = reinterpret_cast<Unit*>(base + c.dst[pair] * page);
   const long long n = page / (long long)sizeof(Unit);
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) dst[i] = src[i];
+  constexpr int DEEP = 4;  // units of a thread that are on their way at a time
+  for (long long i = threadIdx.x; i < n; i += DEEP * 256) {
+    Unit unit[DEEP];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k)
+      if (i + k * 256 < n) unit[k] = src[i + k * 256];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k)
+      if (i + k * 256 < n) dst[i + k * 256] = unit[k];
+  }
 }
 
 int copy_pages(const PageCopies& c, int pairs, int layers, int pools, cudaStream_t st) {

@@ -5,7 +5,7 @@
 // greatest number:
 //   s = bf16((hi - lo) / 15)      m = bf16(lo + 8 s)      c = clamp(round_half_even((x - m) / s), -8, 7) + 8
 // The error of a number is at most s / 2 + 2^-8 |m| (the second part is the rounding of m, not more than the bf16 input's
-// own).  A group whose step is 0 or below 2^-126 holds its least number 32 times; a group with an infinity or a NaN, or
+// own).  A group whose step is 0 or below 2^-120 holds its least number 32 times; a group with an infinity or a NaN, or
 // one that spreads over 2^120 or more, reads back as NaN (m = NaN, s = 0).
 //
 // Memory: codes [slots, heads, D / 2] bytes, lower half of a byte first; (m, s) [slots, heads, D / 32] words, m in the
@@ -37,16 +37,6 @@ __device__ __forceinline__ float add_ieee(float a, float b) {
   asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float min_ieee(float a, float b) {
-  float r;
-  asm("min.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_ieee(float a, float b) {
-  float r;
-  asm("max.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float fma_ieee(float a, float b, float c) {
   float r;
   asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -58,43 +48,54 @@ __device__ __forceinline__ float div_ieee(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t min_bf162(uint32_t a, uint32_t b) {  // of both halves; a NaN wins
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Eight numbers of a lane -> their eight codes (lowest number in the lowest half byte) and the (m, s) word of the group,
 // which four neighbouring lanes share.  Every lane of the warp takes part.
-__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], uint32_t& meta) {
-  float lo = x[0], hi = x[0];
-  uint32_t big = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    lo = min_ieee(lo, x[j]);
-    hi = max_ieee(hi, x[j]);
-    big = max(big, __float_as_uint(x[j]) & 0x7fffffffu);
-  }
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    lo = min_ieee(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_ieee(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-  }
+__device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, uint32_t& meta) {
+  // lower half: the least number, upper half: the greatest with its sign turned
+  const uint32_t a = min_bf162(min_bf162(v.raw.x, v.raw.y), min_bf162(v.raw.z, v.raw.w)), turn = 0x80008000u;
+  const uint32_t b = min_bf162(min_bf162(v.raw.x ^ turn, v.raw.y ^ turn), min_bf162(v.raw.z ^ turn, v.raw.w ^ turn));
+  uint32_t ends = min_bf162(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+  ends = min_bf162(ends, __shfl_xor_sync(0xffffffffu, ends, 1));
+  ends = min_bf162(ends, __shfl_xor_sync(0xffffffffu, ends, 2));
+  const float lo = __uint_as_float(ends << 16), hi = __uint_as_float((ends ^ 0x80000000u) & 0xffff0000u);
   const float spread = sub_ieee(hi, lo);
-  if (big >= 0x7f800000u || spread >= 0x1p120f) {
-    meta = 0x00007fffu;  // m = NaN, s = 0
+  if (!(spread < 0x1p120f)) {  // an infinity, a NaN, or too wide
+    meta = 0x00007fffu;        // m = NaN, s = 0
     return 0x88888888u;
   }
   uint32_t s_bits = __bfloat16_as_ushort(__float2bfloat16_rn(div_ieee(spread, 15.f)));
-  if (s_bits < 0x0080u) s_bits = 0;  // below 2^-126
+  if (s_bits < 0x0380u) s_bits = 0;  // below 2^-120
   const float s = __uint_as_float(s_bits << 16);
   const float mid = s_bits ? add_ieee(lo, 8.f * s) : lo;
   const uint32_t m_bits = __bfloat16_as_ushort(__float2bfloat16_rn(mid));
   const float m = __uint_as_float(m_bits << 16);
   meta = m_bits | (s_bits << 16);
   if (!s_bits) return 0x88888888u;
+  // c' = the nearest whole number to y / s, y = x - m, ties to the even one.  A product with 1 / s is right up to the
+  // neighbour; what it leaves of y is exact (|c' s| has 14 bits at most: |y / s| < 40, as two bf16 numbers of size |m|
+  // that differ do so by 2^-8 |m|) and says which of the two it is.
+  const float inv = div_ieee(1.f, s), half = 0.5f * s;  // s >= 2^-120: neither is subnormal
+  float x[8];
+  v.unpack(x);
   uint32_t word = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = min(7, max(-8, __float2int_rn(div_ieee(sub_ieee(x[j], m), s)))) + 8;
-    word |= (uint32_t)c << (4 * j);
+  for (int j = 7; j >= 0; --j) {
+    const float y = sub_ieee(x[j], m);
+    const float big = fmaf(y, inv, 12582912.f);  // 1.5 2^23 + c': the whole number in the low bits
+    float c = big - 12582912.f;
+    const float rest = fma_ieee(-c, s, y), off = fabsf(rest);
+    const bool odd = __float_as_uint(big) & 1;
+    if (off > half || (off == half && odd)) c += __uint_as_float((__float_as_uint(rest) & 0x80000000u) | 0x3f800000u);
+    c = fminf(fmaxf(c, -8.f), 7.f) + 8388616.f;  // 2^23 + c
+    word = word * 16u + __float_as_uint(c);
   }
-  return word;
+  return word - 0xfb000000u;  // the share of the exponents: sum of 0x4b000000 16^j, as far as it fits
 }
 
 // One row per D / 8 lanes: lane `l` of the row brings its numbers 8 l .. 8 l + 7 (`src`), and the row goes to `codes` /
@@ -105,10 +106,8 @@ __device__ __forceinline__ void kv4_store_row(bool live, bool key, int l, const 
   Vec8<__nv_bfloat16> v;
   v.raw = make_uint4(0, 0, 0, 0);
   if (live) v.load(src + 8 * l);
-  float x[8];
-  v.unpack(x);
   uint32_t ms;
-  const uint32_t word = kv4_quantise(x, ms);
+  const uint32_t word = kv4_quantise(v, ms);
   // a value row's words are made of two half words that two lanes may hold
   const int base = (threadIdx.x & 31) - l;
   uint32_t out = 0;

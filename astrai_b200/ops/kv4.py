@@ -4,7 +4,7 @@ A key or value row of ``D`` numbers (``D`` = 32, 64, 128 or 256) is held in grou
 step ``s`` (bf16 each) and 32 codes ``c`` of four bits, and a number reads back as ``m + s * (c - 8)``: five bits a number,
 3.2 times as many tokens in the memory of a bf16 pool.  With ``lo`` and ``hi`` the group's least and greatest number,
 ``s = bf16((hi - lo) / 15)``, ``m = bf16(lo + 8 s)`` and ``c = clamp(round((x - m) / s), -8, 7) + 8``, so a number is off by
-at most ``s / 2 + 2^-8 |m|``.  A group of equal numbers (or whose step is below 2^-126) holds its least number; a group with
+at most ``s / 2 + 2^-8 |m|``.  A group of equal numbers (or whose step is below 2^-120) holds its least number; a group with
 an infinity or a NaN, or that spreads over 2^120 or more, reads back as NaN.
 
 Pools: codes ``uint8 [slots, heads, D / 2]`` and ``(m, s)`` ``bf16 [slots, heads, D / 32, 2]``, the same shapes for keys and
@@ -17,6 +17,7 @@ the oracle of the tests.  The reference has no quantised cache.
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -28,9 +29,9 @@ HEAD_DIMS = (32, 64, 128, 256)
 GROUP = 32
 
 
-def _ops():
-    native.require()
-    return torch.ops.astrai_b200
+@functools.lru_cache(maxsize=None)
+def _op(name: str):
+    return getattr(native.require(), name).default
 
 
 # ------------------------------------------------------------------------------------------------ plain statements
@@ -71,7 +72,7 @@ def quantize(x: Tensor, keys: bool) -> Tuple[Tensor, Tensor]:
     spread = hi - lo
     bad = ~torch.isfinite(x).all(-1, keepdim=True) | ~(spread < 2.0 ** 120)
     s = (spread / 15).to(torch.bfloat16)
-    s = torch.where(bad | (s.float() < 2.0 ** -126), torch.zeros_like(s), s)
+    s = torch.where(bad | (s.float() < 2.0 ** -120), torch.zeros_like(s), s)
     s32 = s.float()
     m = torch.where(s32 > 0, lo + 8 * s32, lo).to(torch.bfloat16)
     m = torch.where(bad, torch.full_like(m, float("nan")), m)
@@ -94,7 +95,7 @@ def kv4_append_(k: Tensor, v: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: 
     """Store the rows ``k / v [tokens, heads, D]`` into the slots ``loc [tokens]`` (int32 or int64) of the pools.  A slot
     outside the pool is skipped; a slot that occurs twice ends up with a mixture of its rows, so callers name each once."""
     if k_codes.is_cuda:
-        _ops().kv4_append_(k, v, k_codes, k_meta, v_codes, v_meta, loc)
+        _op("kv4_append_")(k, v, k_codes, k_meta, v_codes, v_meta, loc)
         return
     if k.shape != v.shape or k.dim() != 3 or loc.shape != k.shape[:1] or k.shape[1:] != (k_codes.shape[1], 2 * k_codes.shape[2]):
         raise ValueError("kv4_append_: k / v must be [tokens, heads, head_dim] of the pools' heads and head_dim, loc [tokens]")
@@ -108,7 +109,7 @@ def kv4_gather(k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_meta: Tensor,
     """The rows of the slots ``loc [tokens]`` as bf16 ``(k, v)`` ``[tokens, heads, D]``, each number rounded once.  A slot
     outside the pool reads as zeros."""
     if k_codes.is_cuda:
-        return _ops().kv4_gather(k_codes, k_meta, v_codes, v_meta, loc)
+        return _op("kv4_gather")(k_codes, k_meta, v_codes, v_meta, loc)
     ok = _inside(loc, k_codes.shape[0])
     at = torch.where(ok, loc, torch.zeros_like(loc)).long()
     k, v = dequantize(k_codes[at], k_meta[at], True), dequantize(v_codes[at], v_meta[at], False)
@@ -141,9 +142,9 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     if k_codes.is_cuda:
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         o_part, ml_part, counters = workspace if workspace is not None else (None, None, None)
-        _ops().kv4_decode_(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new, scale,
+        _op("kv4_decode_")(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new, scale,
                            max_len, o_part, ml_part, counters, out)
         return out
     b, hq, d = q.shape
@@ -179,7 +180,7 @@ def copy_pages_(pools: Sequence[Tensor], src: Sequence[int], dst: Sequence[int],
     is written: no destination may be a source or occur twice (a source may serve several destinations)."""
     pools = list(pools)
     if pools and pools[0].is_cuda:
-        _ops().copy_pages_(pools, list(src), list(dst), page_size)
+        _op("copy_pages_")(pools, list(src), list(dst), page_size)
         return
     src, dst = [int(p) for p in src], [int(p) for p in dst]
     if not 1 <= len(pools) <= 8:

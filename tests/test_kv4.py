@@ -74,7 +74,7 @@ def test_special_groups():
     x[1, 0, 3] = math.inf
     x[2, 0, 0] = math.nan
     x[3, 0, :2] = torch.tensor([2.0 ** 119, -2.0 ** 119])  # spreads over 2^120
-    x[4, 0, 1] = 2.0 ** -126                               # a step below 2^-126
+    x[4, 0, 1] = 2.0 ** -126                               # a step below 2^-120
     x[5] = torch.tensor([1.0, -1.0] * 16)
     back = kv4.dequantize(*kv4.quantize(x, True), True)
     assert torch.equal(back[0], x[0].float()) and (back[4] == 0).all()
