@@ -45,25 +45,35 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const uint8_t* __restri
                                                          const uint8_t* __restrict__ v_codes, const uint32_t* __restrict__ v_meta,
                                                          const Loc* __restrict__ loc, __nv_bfloat16* __restrict__ k,
                                                          __nv_bfloat16* __restrict__ v, int rows, int heads, long long n_slots) {
-  constexpr int LPR = D / 8, NG = D / 32;
+  constexpr int LPR = D / 8, NG = D / 32, DEEP = 2;  // DEEP: rows of a lane that are on their way at a time
   const int l = threadIdx.x % LPR, g = l >> 2;
-  const int r = (blockIdx.x * 256 + threadIdx.x) / LPR, t = r / heads, h = r - t * heads;
-  const long long slot = r < rows ? (long long)loc[t] : -1;
-  uint32_t kw = 0x88888888u, vw = kw, kms = 0, vms = 0;
-  if (slot >= 0 && slot < n_slots) {
-    const long long at = slot * heads + h;
-    kw = reinterpret_cast<const uint32_t*>(k_codes + at * (D / 2))[kv4_key_word<D>(g, l & 3)];
-    vw = reinterpret_cast<const uint32_t*>(v_codes + at * (D / 2))[l];
-    kms = k_meta[at * NG + g], vms = v_meta[at * NG + g];
+  const int r0 = blockIdx.x * (256 / LPR * DEEP) + threadIdx.x / LPR;
+  uint32_t kw[DEEP], vw[DEEP], kms[DEEP], vms[DEEP];
+#pragma unroll
+  for (int i = 0; i < DEEP; ++i) {
+    const int r = r0 + i * (256 / LPR), t = r / heads, h = r - t * heads;
+    const long long slot = r < rows ? (long long)loc[t] : -1;
+    kw[i] = vw[i] = 0x88888888u, kms[i] = vms[i] = 0;
+    if (slot >= 0 && slot < n_slots) {
+      const long long at = slot * heads + h;
+      kw[i] = reinterpret_cast<const uint32_t*>(k_codes + at * (D / 2))[kv4_key_word<D>(g, l & 3)];
+      vw[i] = reinterpret_cast<const uint32_t*>(v_codes + at * (D / 2))[l];
+      kms[i] = k_meta[at * NG + g], vms[i] = v_meta[at * NG + g];
+    }
   }
   // numbers 8 l .. of a value row are the half words of group g, eighths 2 (l & 3) and the next: with two lanes
   const int base = (threadIdx.x & 31) - l, h0 = kv4_value_half<D>(g, 2 * (l & 3)), h1 = kv4_value_half<D>(g, 2 * (l & 3) + 1);
-  const uint32_t w0 = __shfl_sync(0xffffffffu, vw, base + (h0 >> 1)), w1 = __shfl_sync(0xffffffffu, vw, base + (h1 >> 1));
-  vw = __byte_perm(w0, w1, (h0 & 1 ? 0x0032 : 0x0010) | (h1 & 1 ? 0x7600 : 0x5400));
-  if (r >= rows) return;
-  const long long to = (long long)r * D + 8 * l;
-  *reinterpret_cast<uint4*>(k + to) = kv4_numbers(kw, kms);
-  *reinterpret_cast<uint4*>(v + to) = kv4_numbers(vw, vms);
+#pragma unroll
+  for (int i = 0; i < DEEP; ++i) {
+    const int r = r0 + i * (256 / LPR);
+    const uint32_t w0 = __shfl_sync(0xffffffffu, vw[i], base + (h0 >> 1)), w1 = __shfl_sync(0xffffffffu, vw[i], base + (h1 >> 1));
+    const uint32_t word = __byte_perm(w0, w1, (h0 & 1 ? 0x0032 : 0x0010) | (h1 & 1 ? 0x7600 : 0x5400));
+    if (r < rows) {
+      const long long to = (long long)r * D + 8 * l;
+      __stcs(reinterpret_cast<uint4*>(k + to), kv4_numbers(kw[i], kms[i]));
+      __stcs(reinterpret_cast<uint4*>(v + to), kv4_numbers(word, vms[i]));
+    }
+  }
 }
 
 // Rows of one launch: their lanes are counted in 32 bits.
@@ -105,7 +115,7 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
   const long long step = kKv4Rows / heads;
   for (long long t = 0; t < tokens; t += step) {
     const int rows = (int)((tokens - t < step ? tokens - t : step) * heads);
-    const int grid = ceil_div((long long)rows * (head_dim / 8), 256);
+    const int grid = ceil_div((long long)rows * (head_dim / 8), 512);
     const long long to = t * heads * head_dim;
 #define AB_GATHER(DD, LL)                                                                                                          \
   kv4_gather_kernel<DD, LL><<<grid, 256, 0, st>>>((const uint8_t*)k_codes, (const uint32_t*)k_meta, (const uint8_t*)v_codes,        \

@@ -42,12 +42,6 @@ __device__ __forceinline__ float fma_ieee(float a, float b, float c) {
   asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float div_ieee(float a, float b) {
-  float r;
-  asm("div.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t min_bf162(uint32_t a, uint32_t b) {  // of both halves; a NaN wins
   uint32_t r;
   asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -69,7 +63,9 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, u
     meta = 0x00007fffu;        // m = NaN, s = 0
     return 0x88888888u;
   }
-  uint32_t s_bits = __bfloat16_as_ushort(__float2bfloat16_rn(div_ieee(spread, 15.f)));
+  // spread / 15, rounded once: a product with 1 / 15 and one correction by its remainder (Markstein)
+  const float q = spread * (1.f / 15.f), quotient = fma_ieee(fma_ieee(-q, 15.f, spread), 1.f / 15.f, q);
+  uint32_t s_bits = __bfloat16_as_ushort(__float2bfloat16_rn(quotient));
   if (s_bits < 0x0380u) s_bits = 0;  // below 2^-120
   const float s = __uint_as_float(s_bits << 16);
   const float mid = s_bits ? add_ieee(lo, 8.f * s) : lo;
@@ -80,7 +76,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, u
   // c' = the nearest whole number to y / s, y = x - m, ties to the even one.  A product with 1 / s is right up to the
   // neighbour; what it leaves of y is exact (|c' s| has 14 bits at most: |y / s| < 40, as two bf16 numbers of size |m|
   // that differ do so by 2^-8 |m|) and says which of the two it is.
-  const float inv = div_ieee(1.f, s), half = 0.5f * s;  // s >= 2^-120: neither is subnormal
+  const float inv = 1.f / s, half = 0.5f * s;  // 2^-120 <= s < 2^117: neither is subnormal
   float x[8];
   v.unpack(x);
   uint32_t word = 0;
