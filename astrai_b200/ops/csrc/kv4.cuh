@@ -85,9 +85,9 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, u
     const float y = sub_ieee(x[j], m);
     const float big = fmaf(y, inv, 12582912.f);  // 1.5 2^23 + c': the whole number in the low bits
     float c = big - 12582912.f;
-    const float rest = fma_ieee(-c, s, y), off = fabsf(rest);
-    const bool odd = __float_as_uint(big) & 1;
-    if (off > half || (off == half && odd)) c += __uint_as_float((__float_as_uint(rest) & 0x80000000u) | 0x3f800000u);
+    const float rest = fma_ieee(-c, s, y);
+    const float most = __uint_as_float(__float_as_uint(half) - (__float_as_uint(big) & 1u));  // an odd c' may not have s / 2 left
+    if (fabsf(rest) > most) c += __uint_as_float((__float_as_uint(rest) & 0x80000000u) | 0x3f800000u);
     c = fminf(fmaxf(c, -8.f), 7.f) + 8388616.f;  // 2^23 + c
     word = word * 16u + __float_as_uint(c);
   }
