@@ -148,11 +148,13 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
 // accumulator's rounding.  lo_kg sum(q_hg) is a product of the (m, s) words as they lie in memory with (sum q, -8 sum q)
 // split into three bf16 parts (24 bits).
 //
-// Work: a (request, kv head) is a segment of ceil(len / UNIT) turns of UNIT = 32 W keys and SETUP empty ones (what it costs
-// to begin and end one); the segments of the whole batch, laid end to end, are divided evenly over the CTAs of one wave,
-// whatever the lengths.  A CTA walks its range segment by segment: warp w takes every W-th tile of 32 keys, streams it
-// through a ring of its own in shared memory (cp.async, no barrier between warps), and the warps' sums meet at the end of
-// the segment.  A segment that several CTAs share is joined by the one that finishes last.
+// Work: a request is ceil(len / UNIT) turns of UNIT = 32 W keys and SETUP empty ones (what it costs to begin and end one);
+// the requests of the batch, laid end to end, are divided evenly over groups of CTAs, whatever the lengths.  A group has a
+// CTA for each kv head: the rows of a token's heads lie side by side in memory and are read at about the same time (with
+// the heads' parts cut independently a batch of 16 x 65521 tokens took 211 us).  A CTA walks its range request by request:
+// warp w takes every W-th tile of 32 keys, streams it through a ring of its own in shared memory (cp.async, no barrier
+// between warps), and the warps' sums meet at the end of the request.  What several groups share of a request is joined by
+// the one that finishes last.
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
   if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -247,7 +249,7 @@ template <int N> __device__ __forceinline__ Words<N> lds_words(const uint8_t* p)
 template <int D> struct Kv4Tile {  // a tile of 32 keys in shared memory
   static constexpr int NG = D / 32, KEYS = 32, CODES = KEYS * D / 2, META = KEYS * NG * 4;
   static constexpr int K = 0, V = CODES, KM = 2 * CODES, VM = 2 * CODES + META, BYTES = 2 * (CODES + META);
-  static constexpr int STAGES = 2, STEPS = 3 * 16 * NG * 8, WARP = STAGES * BYTES + STEPS;  // WARP: bytes of a warp
+  static constexpr int STAGES = 2, RING = STAGES * BYTES, STEPS = 3 * 16 * NG * 8, WARP = RING + NG * 512 + STEPS;  // WARP: bytes of a warp
   // 16-byte pieces of a row are swapped by the row's number so that neither the lanes' reads of keys (two rows at a time)
   // nor those of values (four rows, a quarter of each) meet in a bank
   static __device__ __forceinline__ int swap(int r) { return D == 128 ? (r & 2) : D == 256 ? (((r & 1) << 2) | (r & 2)) : 0; }
@@ -263,9 +265,9 @@ template <int D> __device__ __forceinline__ void write_out(const Kv4Attn& p, int
   *reinterpret_cast<uint2*>(p.out + ((long long)seg * p.group + h) * D + d) = make_uint2(bf162_bits(a.x * inv, a.y * inv), bf162_bits(a.z * inv, a.w * inv));
 }
 
-// Joins `n` parts of a segment, `from` the first one's first head: `copies` threads share a number's parts, eight of them on
+// Joins `n` parts of a (request, kv head), `from` the first one's first head and `step` from one to the next: `copies` threads share a number's parts, eight of them on
 // their way at a time, and meet in shared memory.
-template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& p, int seg, long long from, int n, float* meet) {
+template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& p, int seg, long long from, long long step, int n, float* meet) {
   const int items = p.group * (D / 4), copies = max(1, W * 32 / items);
   for (int i = threadIdx.x; i < items * copies; i += W * 32) {
     const int item = i % items, h = item / (D / 4), d = (item % (D / 4)) * 4;
@@ -279,7 +281,7 @@ template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& 
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const bool on = c + j * copies < n;
-        const long long part = from + (on ? c + j * copies : c) * p.group + h;
+        const long long part = from + (on ? c + j * copies : c) * step + h;
         ml[j] = __ldcg(reinterpret_cast<const float2*>(p.ml_part + 2 * part)), v[j] = __ldcg(reinterpret_cast<const float4*>(p.o_part + part * D + d));
         if (!on) ml[j] = make_float2(-INFINITY, 0.f), v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -331,8 +333,9 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   uint8_t* ring = smem + warp * T::WARP;
   // a tile's steps in fp32 as pairs of the two keys that a lane has in a block: [block 4][tig 4][group]; the group's place
   // is turned by the block's number so that the 32 lanes, a key each, write without meeting in a bank
-  Pair* k_step = reinterpret_cast<Pair*>(ring + STAGES * T::BYTES);
+  Pair* k_step = reinterpret_cast<Pair*>(ring + T::RING + NG * 512);
   Pair *v_step = k_step + 16 * NG, *v_low = v_step + 16 * NG;
+  uint32_t* q_frag = reinterpret_cast<uint32_t*>(ring + T::RING);  // the query as operand A, [group][lane][4]
   constexpr int TURN = (NG < 4 ? NG : 4) - 1;
 
   // a length beyond the table row is cut to the row, a row outside the table attends to nothing
@@ -343,10 +346,11 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   };
   auto turns = [&](int len) -> int { return (len + UNIT - 1) / UNIT + SETUP; };
 
-  // CTA i has the turns from cut i to cut i + 1, where cut i lies at turn i base + min(i, extra), moved to the end of its
-  // segment if that is `tol` turns away or less: a cut costs a join.
-  int u, u_end, b, kvh, start, base, extra, n_ctas;  // start: first turn of the current segment (request b, head kvh)
-  auto tol_of = [&](int n) -> int { return min(min(TOL, base >> 1), (n - 1) >> 1); };  // n: turns of the segment
+  // Group i has the turns from cut i to cut i + 1, where cut i lies at turn i base + min(i, extra), moved to the end of its
+  // request if that is `tol` turns away or less: a cut costs a join.
+  const int group = blockIdx.x / p.heads, kvh = blockIdx.x - group * p.heads;
+  int u, u_end, b, start, base, extra;  // start: first turn of the current request b
+  auto tol_of = [&](int n) -> int { return min(min(TOL, base >> 1), (n - 1) >> 1); };  // n: turns of the request
   {
     const int per = (p.batch + W * 32 - 1) / (W * 32);
     const int b0 = threadIdx.x * per;
@@ -366,22 +370,21 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       if (w < warp) before += s_scan[w];
       total += s_scan[w];
     }
-    total = same(total) * p.heads;
-    before *= p.heads;
-    n_ctas = min((int)gridDim.x, (total + SETUP) / (SETUP + 1));
-    if (blockIdx.x >= n_ctas) return;
-    base = total / n_ctas, extra = total % n_ctas;
+    total = same(total);
+    const int n_groups = min((int)gridDim.x / p.heads, (total + SETUP) / (SETUP + 1));
+    if (group >= n_groups) return;
+    base = total / n_groups, extra = total % n_groups;
     int cut[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int i = blockIdx.x + k;
+      const int i = group + k;
       cut[k] = i * base + min(i, extra);
       const int x = min(cut[k], total - 1);
-      if (x >= before && x < before + mine * p.heads) {  // the request that the cut lies in, and the request's first turn
+      if (x >= before && x < before + mine) {  // the request that the cut lies in, and the request's first turn
         int at = before, r = b0;
         if (per > 1) {
           for (;; ++r) {
-            const int here = turns(length(r)) * p.heads;
+            const int here = turns(length(r));
             if (x < at + here) break;
             at += here;
           }
@@ -394,18 +397,13 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
 #pragma unroll
     for (int k = 1; k >= 0; --k) {
       if (cut[k] == total) continue;
-      b = same(s_found[k][0]);
-      const int n = turns(same(length(b))), from = same(s_found[k][1]), tol = tol_of(n);
-      kvh = (cut[k] - from) / n;
-      start = from + kvh * n;
+      b = same(s_found[k][0]), start = same(s_found[k][1]);
+      const int n = turns(same(length(b))), tol = tol_of(n);
       (k ? u_end : u) = cut[k] <= start + tol ? start : cut[k] >= start + n - tol ? start + n : cut[k];
-      if (k == 0 && u == start + n) {  // moved to the start of the next segment
-        start = u;
-        if (++kvh == p.heads) kvh = 0, ++b;
-      }
+      if (k == 0 && u == start + n) start = u, ++b;  // moved to the start of the next request
     }
   }
-  auto cta_of = [&](int x) -> int { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; };
+  auto group_of = [&](int x) -> int { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; };
 
   while (u < u_end) {
     const int len = same(length(b)), row = same(p.rows[b]), n = turns(len), behind = start + n;
@@ -459,7 +457,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         cp_async<PIECE>(to + T::VM, p.v_meta + (uint64_t)at_row + i * (PIECE / 4));
       }
     };
-    uint32_t qa[NG][4], qs[BATCHES][3];
+    uint32_t qs[BATCHES][3];
     float back = 0.f;
     // o: numbers 32 g + 4 gid + 2 i (+ 1: elements 2 and 3) of heads 2 tig and 2 tig + 1; z: sum p lo of head gid
     float o[NG][2][4], mx = -INFINITY;
@@ -520,8 +518,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
             t += __shfl_xor_sync(0xffffffffu, t, 2);
             sums[w] = t * p.scale_log2;
             const float odd = up * 0.0625f;
-            qa[w][0] = half2_bits(x[w][0] * up, x[w][4] * up), qa[w][1] = half2_bits(x[w][1] * odd, x[w][5] * odd);
-            qa[w][2] = half2_bits(x[w][2] * up, x[w][6] * up), qa[w][3] = half2_bits(x[w][3] * odd, x[w][7] * odd);
+            *reinterpret_cast<uint4*>(q_frag + (w * 32 + lane) * 4) = make_uint4(half2_bits(x[w][0] * up, x[w][4] * up), half2_bits(x[w][1] * odd, x[w][5] * odd), half2_bits(x[w][2] * up, x[w][6] * up), half2_bits(x[w][3] * odd, x[w][7] * odd));
           }
 #pragma unroll
           for (int h = 0; h < BATCHES; ++h) {  // lane tig: (sum, -8 sum) of group 4 h + tig, in three parts
@@ -579,30 +576,33 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       // ---- logits of 4 blocks of 8 keys: this lane's head is gid, its keys row_e[0] and row_e[1] of each block
       const float none[4] = {0.f, 0.f, 0.f, 0.f};
       Pair s[4];
+      Pair acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+      for (int w = 0; w < NG; ++w) {
+        const uint4 qw = *reinterpret_cast<const uint4*>(q_frag + (w * 32 + lane) * 4);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int r = 8 * n + key_row;
+          const uint8_t* at = NG >= 4 ? tile + T::K + r * (D / 2) + (((4 * (w / 4) + tig) ^ T::swap(r)) * 16) + (w % 4) * 4 : tile + T::K + r * (D / 2) + tig * NG * 4 + w * 4;
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(at), y = x >> 8;
+          const Pair step = k_step[(4 * n + tig) * NG + (w & ~TURN) + ((w & TURN) ^ (n & TURN))];
+          float part[4];
+          mma_f16(part, qw.x, 0u, qw.y, 0u, x & 0x000f000fu, x & 0x00f000f0u, none);
+          mma_f16(part, qw.z, 0u, qw.w, 0u, y & 0x000f000fu, y & 0x00f000f0u, part);
+          acc[n] = fma2({part[0], part[1]}, step, acc[n]);
+        }
+      }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int r = 8 * n + key_row;
         float term[4] = {0.f, 0.f, 0.f, 0.f};
-        Pair acc = {0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < BATCHES; ++h) {
           const uint32_t word = tig < NB ? *reinterpret_cast<const uint32_t*>(tile + T::KM + (r * NG + h * NB + (tig < NB ? tig : 0)) * 4) : 0u;
           mma_bf16(term, qs[h][0], qs[h][1], word, word, term);
           mma_bf16(term, qs[h][2], 0u, word, 0u, term);
-          Words<NB> codes;
-          if constexpr (NG >= 4) codes = lds_words<NB>(tile + T::K + r * (D / 2) + (((4 * h + tig) ^ T::swap(r)) * 16));
-          else codes = lds_words<NB>(tile + T::K + r * (D / 2) + tig * NB * 4);
-          const Pairs<NB> step = lds_pairs<NB>(k_step + (4 * n + tig) * NG + h * NB);
-#pragma unroll
-          for (int w = 0; w < NB; ++w) {
-            const uint32_t x = codes.w[w], y = x >> 8;
-            float part[4];
-            mma_f16(part, qa[h * NB + w][0], 0u, qa[h * NB + w][1], 0u, x & 0x000f000fu, x & 0x00f000f0u, none);
-            mma_f16(part, qa[h * NB + w][2], 0u, qa[h * NB + w][3], 0u, y & 0x000f000fu, y & 0x00f000f0u, part);
-            acc = fma2({part[0], part[1]}, step.p[w ^ (n & TURN)], acc);
-          }
         }
-        s[n] = fma2(mul2(acc, {back, back}), {p.scale_log2 * 0x1p24f, p.scale_log2 * 0x1p24f}, {term[0], term[1]});
+        s[n] = fma2(mul2(acc[n], {back, back}), {p.scale_log2 * 0x1p24f, p.scale_log2 * 0x1p24f}, {term[0], term[1]});
       }
       if (mask != 0xffffffffu) {
 #pragma unroll
@@ -719,14 +719,14 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         weigh(s_ml[w][h][0], s_ml[w][h][1], *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * T::WARP) + h * D + d), zero, ls, a);
       if (whole) {
         write_out<D>(p, seg, h, d, ls, a);
-      } else {  // part number CTA + segment: no other pair has it
-        const long long part = ((long long)blockIdx.x + seg) * p.group + h;
+      } else {  // part number group + request of the head: no other pair has it
+        const long long part = (((long long)group + b) * p.heads + kvh) * p.group + h;
         *reinterpret_cast<float4*>(p.o_part + part * D + d) = a;
         if (d == 0) p.ml_part[2 * part] = top, p.ml_part[2 * part + 1] = ls;
       }
     }
     if (!whole) {  // the CTA that finishes a shared segment last joins its parts
-      const int tol = tol_of(n), cta0 = cta_of(start + tol), parts = cta_of(behind - 1 - tol) - cta0 + 1;
+      const int tol = tol_of(n), group0 = group_of(start + tol), parts = group_of(behind - 1 - tol) - group0 + 1;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -736,35 +736,36 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       __syncthreads();
       if (s_last) {
         __threadfence();
-        kv4_join<D, W>(p, seg, ((long long)cta0 + seg) * p.group, parts, reinterpret_cast<float*>(smem));
+        kv4_join<D, W>(p, seg, (((long long)group0 + b) * p.heads + kvh) * p.group, (long long)p.heads * p.group, parts, reinterpret_cast<float*>(smem));
       }
     }
     __syncthreads();  // the rings and the sums are free again
 
     u = start = behind;
-    if (++kvh == p.heads) kvh = 0, ++b;
+    ++b;
   }
 }
 
 template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long room, long long max_len, cudaStream_t st) {
   constexpr int bytes = W * Kv4Tile<D>::WARP;
-  static_assert(Kv4Tile<D>::STAGES * Kv4Tile<D>::BYTES >= 8 * D * 4, "a warp's ring holds its sums");
+  static_assert(Kv4Tile<D>::RING >= 8 * D * 4, "a warp's ring holds its sums");
   if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
-  const long long segments = (long long)p.batch * p.heads;
-  if (p.max_ctx > 0x7fffff00 || segments * (p.max_ctx / (32 * W) + 4) > 0x3fffffffLL) return -4;
-  const long long most = segments * ((max_len - 1) / (32 * W) + 1);  // units, if no request is longer
-  long long ctas = 148 * kv4_per_sm<D, W>();
-  if (ctas > room) ctas = room;
-  if (ctas > most) ctas = most;
-  kv4_attn_kernel<D, W><<<(unsigned)ctas, W * 32, bytes, st>>>(p);
+  if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
+  const long long most = p.batch * ((max_len - 1) / (32 * W) + 1);  // units, if no request is longer
+  long long groups = 148 * kv4_per_sm<D, W>() / p.heads;
+  if (groups > room) groups = room;
+  if (groups > most) groups = most;
+  if (groups < 1) groups = 1;
+  if (groups * p.heads > 0x7fffffffLL) return -4;
+  kv4_attn_kernel<D, W><<<(unsigned)(groups * p.heads), W * 32, bytes, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
-// Few segments: the workspace bounds the parts (one for each CTA and segment that meet), so each part is made by more warps.
+// Few requests: the workspace bounds the parts (one for each group and request that meet), so each part is made by more warps.
 template <int D> static int kv4_attn_pick(const Kv4Attn& p, int parts, long long max_len, cudaStream_t st) {
-  const long long room = (long long)p.batch * p.heads * (parts - 1) + 1;
+  const long long room = (long long)p.batch * (parts - 1) + 1;
   if constexpr (D <= 128) {
-    if (room < 148 * 3) return kv4_attn_launch<D, 12>(p, room, max_len, st);
+    if (room < 148 * 3 / p.heads) return kv4_attn_launch<D, 12>(p, room, max_len, st);
   }
   return kv4_attn_launch<D, 4>(p, room, max_len, st);
 }
