@@ -163,17 +163,16 @@ template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const vo
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// d = a b + c; the upper 8 rows of A are a1 / a3
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
-                                        const float (&c)[4]) {
+// d = a b + c; rows 0-7 of A are a.x / a.z, rows 8-15 a.y / a.w
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint4 a, uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint4 a, uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 // two fp32 numbers at a time
 struct Pair { float x, y; };
@@ -249,7 +248,8 @@ template <int N> __device__ __forceinline__ Words<N> lds_words(const uint8_t* p)
 template <int D> struct Kv4Tile {  // a tile of 32 keys in shared memory
   static constexpr int NG = D / 32, KEYS = 32, CODES = KEYS * D / 2, META = KEYS * NG * 4;
   static constexpr int K = 0, V = CODES, KM = 2 * CODES, VM = 2 * CODES + META, BYTES = 2 * (CODES + META);
-  static constexpr int STAGES = 2, RING = STAGES * BYTES, STEPS = 3 * 16 * NG * 8, WARP = RING + NG * 512 + STEPS;  // WARP: bytes of a warp
+  static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4, RING = STAGES * BYTES, QUERY = 512 * (2 * NG + 2 * (NG < 4 ? 1 : NG / 4)), STEPS = 3 * 16 * NG * 8;
+  static constexpr int WARP = RING + STEPS;  // bytes of a warp; the query's are the CTA's  // WARP: bytes of a warp
   // 16-byte pieces of a row are swapped by the row's number so that neither the lanes' reads of keys (two rows at a time)
   // nor those of values (four rows, a quarter of each) meet in a bank
   static __device__ __forceinline__ int swap(int r) { return D == 128 ? (r & 2) : D == 256 ? (((r & 1) << 2) | (r & 2)) : 0; }
@@ -333,9 +333,10 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   uint8_t* ring = smem + warp * T::WARP;
   // a tile's steps in fp32 as pairs of the two keys that a lane has in a block: [block 4][tig 4][group]; the group's place
   // is turned by the block's number so that the 32 lanes, a key each, write without meeting in a bank
-  Pair* k_step = reinterpret_cast<Pair*>(ring + T::RING + NG * 512);
+  Pair* k_step = reinterpret_cast<Pair*>(ring + T::RING);
   Pair *v_step = k_step + 16 * NG, *v_low = v_step + 16 * NG;
-  uint32_t* q_frag = reinterpret_cast<uint32_t*>(ring + T::RING);  // the query as operand A, [group][lane][4]
+  // the query as operand A, a register quad of each lane at a time: two steps of every group, two of (sum q, -8 sum q)
+  uint4* q_frag = reinterpret_cast<uint4*>(smem + W * T::WARP);
   constexpr int TURN = (NG < 4 ? NG : 4) - 1;
 
   // a length beyond the table row is cut to the row, a row outside the table attends to nothing
@@ -457,7 +458,6 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         cp_async<PIECE>(to + T::VM, p.v_meta + (uint64_t)at_row + i * (PIECE / 4));
       }
     };
-    uint32_t qs[BATCHES][3];
     float back = 0.f;
     // o: numbers 32 g + 4 gid + 2 i (+ 1: elements 2 and 3) of heads 2 tig and 2 tig + 1; z: sum p lo of head gid
     float o[NG][2][4], mx = -INFINITY;
@@ -470,75 +470,77 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
     }
     const int key_row = (gid & 1) ? ((gid >> 1) ^ 1) + 4 : gid >> 1;  // row of a block of 8 keys that column gid stands for
     const int row_e[2] = {tig, (tig ^ 1) + 4};                        // rows of columns 2 tig and 2 tig + 1
-    int ahead = key, slot = slot_of(key), stage = 0;
-    // turn t copies tile t and computes tile t - (STAGES - 1)
-    for (int t = 0;; ++t) {
-      if (t >= STAGES - 1) {
-        if (key >= key_end) break;
-        cp_wait<STAGES - 2>();
-        __syncwarp();
-      }
-      if (ahead < key_end) {  // into the stage that the previous turn has read
+    int ahead = key, slot = slot_of(key);
+    auto copy_next = [&](int into) {
+      if (ahead < key_end) {
         const int cur = slot;
         slot = slot_of(ahead + UNIT);
-        issue(ahead, cur, t % STAGES);
+        issue(ahead, cur, into);
         ahead += UNIT;
       }
       cp_commit();
-      if (t < STAGES - 1) continue;
-      if (t == STAGES - 1) {
-        // ---- the query as operand A: row gid = head, numbers 32 w + 8 tig + (0 4 | 1 5 | 2 6 | 3 7) as pairs
-        {
-          float x[NG][8], big = 0.f;
-          const bool on = gid < p.group;
-          const __nv_bfloat16* src = p.q + (((long long)b * p.heads + kvh) * p.group + (on ? gid : 0)) * D + 8 * tig;
+    };
+#pragma unroll 1
+    for (int t = 0; t < STAGES - 1; ++t) copy_next(t);
+    // ---- the query as operand A: row gid = head, numbers 32 w + 8 tig + (0 4 | 1 5 | 2 6 | 3 7) as pairs
+    {
+      float x[NG][8], big = 0.f;
+      const bool on = gid < p.group;
+      const __nv_bfloat16* src = p.q + (((long long)b * p.heads + kvh) * p.group + (on ? gid : 0)) * D + 8 * tig;
 #pragma unroll
-          for (int w = 0; w < NG; ++w) {
-            Vec8<__nv_bfloat16> v;
-            v.load(src + 32 * w);
-            v.unpack(x[w]);
+      for (int w = 0; w < NG; ++w) {
+        Vec8<__nv_bfloat16> v;
+        v.load(src + 32 * w);
+        v.unpack(x[w]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (!on) x[w][j] = 0.f;
-              big = fmaxf(big, fabsf(x[w][j]));
-            }
-          }
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-          const int e = min(126, 140 - (int)(__float_as_uint(big) >> 23));
-          const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-          back = __uint_as_float((uint32_t)(127 - e) << 23);
-          float sums[NG];
-#pragma unroll
-          for (int w = 0; w < NG; ++w) {
-            float t = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t += x[w][j];
-            t += __shfl_xor_sync(0xffffffffu, t, 1);
-            t += __shfl_xor_sync(0xffffffffu, t, 2);
-            sums[w] = t * p.scale_log2;
-            const float odd = up * 0.0625f;
-            *reinterpret_cast<uint4*>(q_frag + (w * 32 + lane) * 4) = make_uint4(half2_bits(x[w][0] * up, x[w][4] * up), half2_bits(x[w][1] * odd, x[w][5] * odd), half2_bits(x[w][2] * up, x[w][6] * up), half2_bits(x[w][3] * odd, x[w][7] * odd));
-          }
-#pragma unroll
-          for (int h = 0; h < BATCHES; ++h) {  // lane tig: (sum, -8 sum) of group 4 h + tig, in three parts
-            float t = 0.f;
-#pragma unroll
-            for (int w = 0; w < NB; ++w) t = tig == w ? sums[h * NB + w] : t;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-              const float part = __bfloat162float(__float2bfloat16_rn(t));
-              const __nv_bfloat162 pair = __floats2bfloat162_rn(part, -8.f * part);
-              qs[h][i] = *reinterpret_cast<const uint32_t*>(&pair);
-              t -= part;
-            }
-          }
+        for (int j = 0; j < 8; ++j) {
+          if (!on) x[w][j] = 0.f;
+          big = fmaxf(big, fabsf(x[w][j]));
         }
       }
-      const uint8_t* tile = ring + stage * T::BYTES;
-      const uint32_t mask = same(s_mask[warp][stage]);
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-      key += UNIT;
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const int e = min(126, 140 - (int)(__float_as_uint(big) >> 23));
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+      back = __uint_as_float((uint32_t)(127 - e) << 23);
+      float sums[NG];
+#pragma unroll
+      for (int w = 0; w < NG; ++w) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t += x[w][j];
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        sums[w] = t * p.scale_log2;
+        const float odd = up * 0.0625f;
+        if (w % W != warp) continue;  // every warp has all of them, each brings its share
+        q_frag[(2 * w) * 32 + lane] = make_uint4(half2_bits(x[w][0] * up, x[w][4] * up), 0u, half2_bits(x[w][1] * odd, x[w][5] * odd), 0u);
+        q_frag[(2 * w + 1) * 32 + lane] = make_uint4(half2_bits(x[w][2] * up, x[w][6] * up), 0u, half2_bits(x[w][3] * odd, x[w][7] * odd), 0u);
+      }
+#pragma unroll
+      for (int h = 0; h < BATCHES; ++h) {  // lane tig: (sum, -8 sum) of group 4 h + tig, in three parts
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < NB; ++w) t = tig == w ? sums[h * NB + w] : t;
+        uint32_t parts[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const float part = __bfloat162float(__float2bfloat16_rn(t));
+          parts[i] = bf162_bits(part, -8.f * part);
+          t -= part;
+        }
+        if (warp != W - 1) continue;
+        q_frag[(2 * NG + 2 * h) * 32 + lane] = make_uint4(parts[0], 0u, parts[1], 0u);
+        q_frag[(2 * NG + 2 * h + 1) * 32 + lane] = make_uint4(parts[2], 0u, 0u, 0u);
+      }
+    }
+    __syncthreads();
+    for (int t = 0; key < key_end; t = t + 1 == STAGES ? 0 : t + 1, key += UNIT) {
+      cp_wait<STAGES - 2>();
+      __syncwarp();
+      copy_next(t == 0 ? STAGES - 1 : t - 1);  // into the stage that the previous turn has read
+      const uint8_t* tile = ring + t * T::BYTES;
+      const uint32_t mask = same(s_mask[warp][t]);
       if (mask == 0) continue;
       // ---- steps: lane = key
       float down;
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       Pair acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
-        const uint4 qw = *reinterpret_cast<const uint4*>(q_frag + (w * 32 + lane) * 4);
+        const uint4 q0 = q_frag[(2 * w) * 32 + lane], q1 = q_frag[(2 * w + 1) * 32 + lane];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const int r = 8 * n + key_row;
@@ -587,23 +589,25 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
           const uint32_t x = *reinterpret_cast<const uint32_t*>(at), y = x >> 8;
           const Pair step = k_step[(4 * n + tig) * NG + (w & ~TURN) + ((w & TURN) ^ (n & TURN))];
           float part[4];
-          mma_f16(part, qw.x, 0u, qw.y, 0u, x & 0x000f000fu, x & 0x00f000f0u, none);
-          mma_f16(part, qw.z, 0u, qw.w, 0u, y & 0x000f000fu, y & 0x00f000f0u, part);
+          mma_f16(part, q0, x & 0x000f000fu, x & 0x00f000f0u, none);
+          mma_f16(part, q1, y & 0x000f000fu, y & 0x00f000f0u, part);
           acc[n] = fma2({part[0], part[1]}, step, acc[n]);
         }
       }
+      float term[4][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int r = 8 * n + key_row;
-        float term[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < BATCHES; ++h) {
+        const uint4 q0 = q_frag[(2 * NG + 2 * h) * 32 + lane], q1 = q_frag[(2 * NG + 2 * h + 1) * 32 + lane];
 #pragma unroll
-        for (int h = 0; h < BATCHES; ++h) {
-          const uint32_t word = tig < NB ? *reinterpret_cast<const uint32_t*>(tile + T::KM + (r * NG + h * NB + (tig < NB ? tig : 0)) * 4) : 0u;
-          mma_bf16(term, qs[h][0], qs[h][1], word, word, term);
-          mma_bf16(term, qs[h][2], 0u, word, 0u, term);
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t word = tig < NB ? *reinterpret_cast<const uint32_t*>(tile + T::KM + ((8 * n + key_row) * NG + h * NB + (tig < NB ? tig : 0)) * 4) : 0u;
+          if (h == 0) mma_bf16(term[n], q0, word, word, none);
+          else mma_bf16(term[n], q0, word, word, term[n]);
+          mma_bf16(term[n], q1, word, 0u, term[n]);
         }
-        s[n] = fma2(mul2(acc[n], {back, back}), {p.scale_log2 * 0x1p24f, p.scale_log2 * 0x1p24f}, {term[0], term[1]});
       }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) s[n] = fma2(mul2(acc[n], {back, back}), {p.scale_log2 * 0x1p24f, p.scale_log2 * 0x1p24f}, {term[n][0], term[n][1]});
       if (mask != 0xffffffffu) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -673,8 +677,9 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const uint32_t x = i ? pair[2 * j] >> 8 : pair[2 * j], y = i ? pair[2 * j + 1] >> 8 : pair[2 * j + 1];
-              if (j == 0) mma_f16(t, x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[0][g], pb[1][g], none);
-              else mma_f16(t, x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[2][g], pb[3][g], t);
+              const uint4 a = make_uint4(x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u);
+              if (j == 0) mma_f16(t, a, pb[0][g], pb[1][g], none);
+              else mma_f16(t, a, pb[2][g], pb[3][g], t);
             }
             float(&to)[4] = o[h * PB + g][i];
             const Pair lo = fma2({t[0], t[1]}, {down, down}, {to[0], to[1]});
@@ -747,7 +752,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
 }
 
 template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long room, long long max_len, cudaStream_t st) {
-  constexpr int bytes = W * Kv4Tile<D>::WARP;
+  constexpr int bytes = W * Kv4Tile<D>::WARP + Kv4Tile<D>::QUERY;
   static_assert(Kv4Tile<D>::RING >= 8 * D * 4, "a warp's ring holds its sums");
   if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
   if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
