@@ -105,7 +105,7 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
         if kv_cache.four_bit:
             out = kv_cache.decode_out[:b] if kv_cache.decode_out is not None else None
             return kv4.kv4_decode(q, *kv_cache.layer_pools(layer_id), kv_cache.req_to_token, kv_cache.req_pool_indices,
-                                  kv_cache.seq_lens, k_new=k, v_new=v, scale=scale, out=out,
+                                  kv_cache.seq_lens, k_new=k, v_new=v, scale=scale, max_len=kv_cache.max_len, out=out,
                                   workspace=(kv_cache.decode_o_part, kv_cache.decode_ml_part, kv_cache.decode_counters))
         splits = kv_cache.decode_splits or int(torch.ops.astrai_b200.paged_decode_splits(
             b, kv_cache.k_buffer.shape[2], max(kv_cache.max_len, 1), kv_cache.decode_o_part.shape[2]))
