@@ -249,7 +249,9 @@ template <int D> struct Kv4Tile {  // a tile of 32 keys in shared memory
   static constexpr int NG = D / 32, KEYS = 32, CODES = KEYS * D / 2, META = KEYS * NG * 4;
   static constexpr int K = 0, V = CODES, KM = 2 * CODES, VM = 2 * CODES + META, BYTES = 2 * (CODES + META);
   static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4, RING = STAGES * BYTES, QUERY = 512 * (2 * NG + 2 * (NG < 4 ? 1 : NG / 4)), STEPS = 3 * 16 * NG * 8;
-  static constexpr int WARP = RING + STEPS;  // bytes of a warp; the query's are the CTA's  // WARP: bytes of a warp
+  // behind a warp's ring: a tile's steps, or four heads of its sums when they meet those of the other warps
+  static constexpr int SPACE = STEPS > 16 * D ? (STEPS > 1024 ? STEPS : 1024) : (16 * D > 1024 ? 16 * D : 1024);
+  static constexpr int WARP = RING + SPACE;  // bytes of a warp; the query's are the CTA's
   // 16-byte pieces of a row are swapped by the row's number so that neither the lanes' reads of keys (two rows at a time)
   // nor those of values (four rows, a quarter of each) meet in a bank
   static __device__ __forceinline__ int swap(int r) { return D == 128 ? (r & 2) : D == 256 ? (((r & 1) << 2) | (r & 2)) : 0; }
@@ -267,8 +269,9 @@ template <int D> __device__ __forceinline__ void write_out(const Kv4Attn& p, int
 
 // Joins `n` parts of a (request, kv head), `from` the first one's first head and `step` from one to the next: `copies` threads share a number's parts, eight of them on
 // their way at a time, and meet in shared memory.
-template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& p, int seg, long long from, long long step, int n, float* meet) {
+template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& p, int seg, long long from, long long step, int n, uint8_t* smem) {
   const int items = p.group * (D / 4), copies = max(1, W * 32 / items);
+  auto meet = [&](int i) -> float* { return reinterpret_cast<float*>(smem + (i >> 5) * Kv4Tile<D>::WARP + Kv4Tile<D>::RING) + (i & 31) * 8; };
   for (int i = threadIdx.x; i < items * copies; i += W * 32) {
     const int item = i % items, h = item / (D / 4), d = (item % (D / 4)) * 4;
     float top = -INFINITY, l = 0.f;
@@ -296,8 +299,8 @@ template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& 
     if (copies == 1) {
       write_out<D>(p, seg, h, d, l, a);
     } else {
-      *reinterpret_cast<float4*>(meet + i * 8) = a;
-      meet[i * 8 + 4] = top, meet[i * 8 + 5] = l;
+      *reinterpret_cast<float4*>(meet(i)) = a;
+      meet(i)[4] = top, meet(i)[5] = l;
     }
   }
   if (copies == 1) return;
@@ -305,10 +308,10 @@ template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& 
   for (int i = threadIdx.x; i < items; i += W * 32) {
     float top = -INFINITY, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < copies; ++c) top = fmaxf(top, meet[(c * items + i) * 8 + 4]);
+    for (int c = 0; c < copies; ++c) top = fmaxf(top, meet(c * items + i)[4]);
     const float zero = top == -INFINITY ? 0.f : top;
     for (int c = 0; c < copies; ++c) {
-      const float* at = meet + (c * items + i) * 8;
+      const float* at = meet(c * items + i);
       weigh(at[4], at[5], *reinterpret_cast<const float4*>(at), zero, l, a);
     }
     write_out<D>(p, seg, i / (D / 4), (i % (D / 4)) * 4, l, a);
@@ -337,6 +340,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   // a tile's steps in fp32 as pairs of the two keys that a lane has in a block: [block 4][tig 4][group]; the group's place
   // is turned by the block's number so that the 32 lanes, a key each, write without meeting in a bank
   Pair* k_step = reinterpret_cast<Pair*>(ring + T::RING);
+  float* space = reinterpret_cast<float*>(ring + T::RING);
   Pair *v_step = k_step + 16 * NG, *v_low = v_step + 16 * NG;
   // the query as operand A, a register quad of each lane at a time: two steps of every group, two of (sum q, -8 sum q)
   uint4* q_frag = reinterpret_cast<uint4*>(smem + W * T::WARP);
@@ -409,87 +413,164 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   }
   auto group_of = [&](int x) -> int { return x < extra * (base + 1) ? x / (base + 1) : extra + (x - extra * (base + 1)) / base; };
 
-  while (u < u_end) {
-    const int len = same(length(b)), row = same(p.rows[b]), n = turns(len), behind = start + n;
-    const int seg = b * p.heads + kvh, stop = min(u_end, behind);
-    const int key_end = stop == behind ? len : max(0, stop - start - SETUP) * UNIT;
-    int key = max(0, u - start - SETUP) * UNIT + warp * 32;  // first key of this warp's next tile
+  // A request, and what this CTA has of it: the keys up to key_end; `key` is the first one of this warp's next tile.
+  struct Part { int b, row, len, start, behind, key, key_end; };
+  Part cur{}, next{};
+  auto enter = [&](Part& r, int request, int first) {
+    r.b = request, r.start = first;
+    r.len = same(length(request)), r.row = same(p.rows[request]);
+    r.behind = first + turns(r.len);
+    r.key_end = u_end >= r.behind ? r.len : max(0, u_end - first - SETUP) * UNIT;
+    r.key = max(0, u - first - SETUP) * UNIT + warp * 32;
+  };
 
-    // ---- copies: a tile's slots, then its rows.  A key whose slot is outside the pool takes the row of one that is not
-    // (nothing, if there is none): its weight will be zero, but what it is multiplied with has to be a number.
-    auto slot_of = [&](int k0) -> int {
-      const int s = k0 + lane < key_end ? p.table[(long long)row * p.max_ctx + k0 + lane] : -1;
-      return s < p.n_slots ? s : -1;
-    };
-    auto issue = [&](int k0, int slot, int stage) {
-      if (p.k_new != nullptr && k0 + 32 >= len) {  // the step's own rows: stored before they are read
-        const int dst = __shfl_sync(0xffffffffu, slot, (len - 1) & 31);
-        constexpr int LPR = D / 8;
-        const long long to = (long long)max(dst, 0) * p.heads + kvh, from = ((long long)b * p.heads + kvh) * D;
+  // ---- copies: a tile's slots, then its rows.  A key whose slot is outside the pool takes the row of one that is not
+  // (nothing, if there is none): its weight will be zero, but what it is multiplied with has to be a number.
+  auto slot_of = [&](const Part& r, int k0) -> int {
+    const int s = k0 + lane < r.key_end ? p.table[(long long)r.row * p.max_ctx + k0 + lane] : -1;
+    return s < p.n_slots ? s : -1;
+  };
+  auto issue = [&](const Part& r, int k0, int slot, int stage) {
+    if (p.k_new != nullptr && k0 + 32 >= r.len) {  // the step's own rows: stored before they are read
+      const int dst = __shfl_sync(0xffffffffu, slot, (r.len - 1) & 31);
+      constexpr int LPR = D / 8;
+      const long long to = (long long)max(dst, 0) * p.heads + kvh, from = ((long long)r.b * p.heads + kvh) * D;
 #pragma unroll 1
-        for (int pass = 0; pass < (D == 256 ? 2 : 1); ++pass) {
-          const int which = D == 256 ? pass : lane / LPR;
-          kv4_store_row<D>(dst >= 0 && which < 2, which == 0, lane % LPR, (which == 0 ? p.k_new : p.v_new) + from,
-                           (which == 0 ? p.k_codes : p.v_codes) + to * (D / 2), (which == 0 ? p.k_meta : p.v_meta) + to * NG);
-        }
-        __threadfence();
-        __syncwarp();
+      for (int pass = 0; pass < (D == 256 ? 2 : 1); ++pass) {
+        const int which = D == 256 ? pass : lane / LPR;
+        kv4_store_row<D>(dst >= 0 && which < 2, which == 0, lane % LPR, (which == 0 ? p.k_new : p.v_new) + from,
+                         (which == 0 ? p.k_codes : p.v_codes) + to * (D / 2), (which == 0 ? p.k_meta : p.v_meta) + to * NG);
       }
-      const uint32_t mask = __ballot_sync(0xffffffffu, slot >= 0);
-      if (lane == 0) s_mask[warp][stage] = mask;
-      if (mask == 0) return;
-      if (mask != 0xffffffffu) {
-        const int other = __shfl_sync(0xffffffffu, slot, __ffs(mask) - 1);
-        if (slot < 0) slot = other;
-      }
-      // a row's codes are NG pieces of 16 bytes, its middles and steps NG words: one number counts both
-      const uint32_t at_row = ((uint32_t)slot * (uint32_t)p.heads + (uint32_t)kvh) * NG;
-      const uint32_t at = smem_addr(ring + stage * T::BYTES);
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int r = i * (32 / NG) + lane / NG;
-        const uint32_t from = __shfl_sync(0xffffffffu, at_row, r) + lane % NG;
-        const uint32_t to = at + r * (D / 2) + (((lane % NG) ^ T::swap(r)) * 16);
-        cp_async<16>(to + T::K, p.k_codes + (uint64_t)from * 16);
-        cp_async<16>(to + T::V, p.v_codes + (uint64_t)from * 16);
-      }
-      constexpr int PIECE = NG < 4 ? NG * 4 : 16;  // bytes of the middles and steps that one copy takes
-#pragma unroll
-      for (int i = 0; i < NG * 4 / PIECE; ++i) {
-        const uint32_t to = at + lane * NG * 4 + i * PIECE;
-        cp_async<PIECE>(to + T::KM, p.k_meta + (uint64_t)at_row + i * (PIECE / 4));
-        cp_async<PIECE>(to + T::VM, p.v_meta + (uint64_t)at_row + i * (PIECE / 4));
-      }
-    };
-    float back = 0.f;
-    // o: numbers 32 g + 4 gid + 2 i (+ 1: elements 2 and 3) of heads 2 tig and 2 tig + 1; z: sum p lo of head gid
-    float o[NG][2][4], mx = -INFINITY;
-    Pair z[NG], sum = {0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      z[g] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[g][i >> 2][i & 3] = 0.f;
+      __threadfence();
+      __syncwarp();
     }
-    const int key_row = (gid & 1) ? ((gid >> 1) ^ 1) + 4 : gid >> 1;  // row of a block of 8 keys that column gid stands for
-    const int row_e[2] = {tig, (tig ^ 1) + 4};                        // rows of columns 2 tig and 2 tig + 1
-    int ahead = key, slot = slot_of(key);
-    auto copy_next = [&](int into) {
-      if (ahead < key_end) {
-        const int cur = slot;
-        slot = slot_of(ahead + UNIT);
-        issue(ahead, cur, into);
-        ahead += UNIT;
-      }
-      cp_commit();
-    };
+    const uint32_t mask = __ballot_sync(0xffffffffu, slot >= 0);
+    if (lane == 0) s_mask[warp][stage] = mask;
+    if (mask == 0) return;
+    if (mask != 0xffffffffu) {
+      const int other = __shfl_sync(0xffffffffu, slot, __ffs(mask) - 1);
+      if (slot < 0) slot = other;
+    }
+    // a row's codes are NG pieces of 16 bytes, its middles and steps NG words: one number counts both
+    const uint32_t at_row = ((uint32_t)slot * (uint32_t)p.heads + (uint32_t)kvh) * NG;
+    const uint32_t at = smem_addr(ring + stage * T::BYTES);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const int row = i * (32 / NG) + lane / NG;
+      const uint32_t from = __shfl_sync(0xffffffffu, at_row, row) + lane % NG;
+      const uint32_t to = at + row * (D / 2) + (((lane % NG) ^ T::swap(row)) * 16);
+      cp_async<16>(to + T::K, p.k_codes + (uint64_t)from * 16);
+      cp_async<16>(to + T::V, p.v_codes + (uint64_t)from * 16);
+    }
+    constexpr int PIECE = NG < 4 ? NG * 4 : 16;  // bytes of the middles and steps that one copy takes
+#pragma unroll
+    for (int i = 0; i < NG * 4 / PIECE; ++i) {
+      const uint32_t to = at + lane * NG * 4 + i * PIECE;
+      cp_async<PIECE>(to + T::KM, p.k_meta + (uint64_t)at_row + i * (PIECE / 4));
+      cp_async<PIECE>(to + T::VM, p.v_meta + (uint64_t)at_row + i * (PIECE / 4));
+    }
+  };
+  int ahead = 0, slot = -1;  // the next tile to copy, and its slots
+  auto copy_next = [&](const Part& r, int stage) {
+    if (ahead < r.key_end) {
+      const int now = slot;
+      slot = slot_of(r, ahead + UNIT);
+      issue(r, ahead, now, stage);
+      ahead += UNIT;
+    }
+    cp_commit();
+  };
+
+  float back = 0.f;  // undoes the query's power of two
+  // o: numbers 32 g + 4 gid + 2 i (+ 1: elements 2 and 3) of heads 2 tig and 2 tig + 1; z: sum p lo of head gid
+  float o[NG][2][4], mx = -INFINITY;
+  Pair z[NG], sum = {0.f, 0.f};
+  const int key_row = (gid & 1) ? ((gid >> 1) ^ 1) + 4 : gid >> 1;  // row of a block of 8 keys that column gid stands for
+  const int row_e[2] = {tig, (tig ^ 1) + 4};                        // rows of columns 2 tig and 2 tig + 1
+  bool began = false, going = false;  // going: a request (cur) is in hand, its tiles are done; began: it began in this CTA
+  if (u < u_end) enter(next, b, start);
+  for (;;) {
+    // ---- the first tiles of the next request are on their way while the one in hand ends
+    const bool more = going ? cur.behind < u_end : u < u_end;
+    if (more) {
+      if (going) u = cur.behind, enter(next, cur.b + 1, cur.behind);
+      ahead = next.key, slot = slot_of(next, ahead);
 #pragma unroll 1
-    for (int t = 0; t < STAGES - 1; ++t) copy_next(t);
+      for (int t = 0; t < STAGES - 1; ++t) copy_next(next, t);
+    }
+    if (going) {
+      // ---- the warps' sums meet, four heads at a time
+      const int seg = cur.b * p.heads + kvh;
+      const bool whole = began && cur.behind <= u_end;
+      float l = sum.x + sum.y;
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (tig == 0) s_ml[warp][gid][0] = mx, s_ml[warp][gid][1] = l;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float zz = z[g].x + z[g].y;
+        zz += __shfl_xor_sync(0xffffffffu, zz, 1);
+        zz += __shfl_xor_sync(0xffffffffu, zz, 2);
+        const float z0 = __shfl_sync(0xffffffffu, zz, 8 * tig), z1 = __shfl_sync(0xffffffffu, zz, 8 * tig + 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[g][i][0] += z0, o[g][i][1] += z1, o[g][i][2] += z0, o[g][i][3] += z1;
+      }
+#pragma unroll 1
+      for (int h0 = 0; h0 < p.group; h0 += 4) {
+        if ((tig & 2) * 2 == h0) {  // heads 2 tig and 2 tig + 1; numbers 32 g + 4 gid .. + 3
+          float* to = space + (tig & 1) * 2 * D + 4 * gid;
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *reinterpret_cast<float4*>(to + h * D + 32 * g) = make_float4(o[g][0][h], o[g][0][2 + h], o[g][1][h], o[g][1][2 + h]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < min(4, p.group - h0) * (D / 4); i += W * 32) {
+          const int h = h0 + i / (D / 4), d = (i % (D / 4)) * 4;
+          float top = -INFINITY, ls = 0.f;
+#pragma unroll
+          for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][h][0]);
+          const float zero = top == -INFINITY ? 0.f : top;
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            weigh(s_ml[w][h][0], s_ml[w][h][1], *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * T::WARP + T::RING) + (h - h0) * D + d), zero, ls, a);
+          if (whole) {
+            write_out<D>(p, seg, h, d, ls, a);
+          } else {  // part number group + request of the head: no other pair has it
+            const long long part = (((long long)group + cur.b) * p.heads + kvh) * p.group + h;
+            *reinterpret_cast<float4*>(p.o_part + part * D + d) = a;
+            if (d == 0) p.ml_part[2 * part] = top, p.ml_part[2 * part + 1] = ls;
+          }
+        }
+        __syncthreads();
+      }
+      if (!whole) {  // the CTA that finishes a shared request last joins its parts
+        const int tol = tol_of(cur.behind - cur.start), group0 = group_of(cur.start + tol), parts = group_of(cur.behind - 1 - tol) - group0 + 1;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          s_last = atomicAdd(&p.counters[seg], 1) == parts - 1;
+          if (s_last) p.counters[seg] = 0;  // ready for the next launch
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          kv4_join<D, W>(p, seg, (((long long)group0 + cur.b) * p.heads + kvh) * p.group, (long long)p.heads * p.group, parts, smem);
+          __syncthreads();
+        }
+      }
+    }
+    if (!more) break;
+    began = u <= next.start;
+    cur = next;
+    going = true;
     // ---- the query as operand A: row gid = head, numbers 32 w + 8 tig + (0 4 | 1 5 | 2 6 | 3 7) as pairs
     {
       float x[NG][8], big = 0.f;
       const bool on = gid < p.group;
-      const __nv_bfloat16* src = p.q + (((long long)b * p.heads + kvh) * p.group + (on ? gid : 0)) * D + 8 * tig;
+      const __nv_bfloat16* src = p.q + (((long long)cur.b * p.heads + kvh) * p.group + (on ? gid : 0)) * D + 8 * tig;
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
         Vec8<__nv_bfloat16> v;
@@ -537,11 +618,18 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         q_frag[(2 * NG + 2 * h + 1) * 32 + lane] = make_uint4(parts[2], 0u, 0u, 0u);
       }
     }
+    mx = -INFINITY, sum = {0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      z[g] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[g][i >> 2][i & 3] = 0.f;
+    }
     __syncthreads();
-    for (int t = 0; key < key_end; t = t + 1 == STAGES ? 0 : t + 1, key += UNIT) {
+    for (int t = 0; cur.key < cur.key_end; t = t + 1 == STAGES ? 0 : t + 1, cur.key += UNIT) {
       cp_wait<STAGES - 2>();
       __syncwarp();
-      copy_next(t == 0 ? STAGES - 1 : t - 1);  // into the stage that the previous turn has read
+      copy_next(cur, t == 0 ? STAGES - 1 : t - 1);  // into the stage that the previous turn has read
       const uint8_t* tile = ring + t * T::BYTES;
       const uint32_t mask = same(s_mask[warp][t]);
       if (mask == 0) continue;
@@ -692,71 +780,13 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         }
       }
     }
-
-    // ---- the warps' sums meet: out of each warp [8 heads][D] in its own ring
-    float* mine = reinterpret_cast<float*>(ring);
-    float l = sum.x + sum.y;
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    cp_wait<0>();
-    __syncwarp();
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float zz = z[g].x + z[g].y;
-      zz += __shfl_xor_sync(0xffffffffu, zz, 1);
-      zz += __shfl_xor_sync(0xffffffffu, zz, 2);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // heads 2 tig and 2 tig + 1; numbers 32 g + 4 gid .. + 3
-        const float zh = __shfl_sync(0xffffffffu, zz, 8 * tig + 4 * h);
-        *reinterpret_cast<float4*>(mine + (2 * tig + h) * D + 32 * g + 4 * gid) =
-            make_float4(o[g][0][h] + zh, o[g][0][2 + h] + zh, o[g][1][h] + zh, o[g][1][2 + h] + zh);
-      }
-    }
-    if (tig == 0) s_ml[warp][gid][0] = mx, s_ml[warp][gid][1] = l;
-    __syncthreads();
-    const bool whole = u <= start && stop == behind;
-    for (int i = threadIdx.x; i < p.group * (D / 4); i += W * 32) {
-      const int h = i / (D / 4), d = (i % (D / 4)) * 4;
-      float top = -INFINITY, ls = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][h][0]);
-      const float zero = top == -INFINITY ? 0.f : top;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-        weigh(s_ml[w][h][0], s_ml[w][h][1], *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * T::WARP) + h * D + d), zero, ls, a);
-      if (whole) {
-        write_out<D>(p, seg, h, d, ls, a);
-      } else {  // part number group + request of the head: no other pair has it
-        const long long part = (((long long)group + b) * p.heads + kvh) * p.group + h;
-        *reinterpret_cast<float4*>(p.o_part + part * D + d) = a;
-        if (d == 0) p.ml_part[2 * part] = top, p.ml_part[2 * part + 1] = ls;
-      }
-    }
-    if (!whole) {  // the CTA that finishes a shared segment last joins its parts
-      const int tol = tol_of(n), group0 = group_of(start + tol), parts = group_of(behind - 1 - tol) - group0 + 1;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        s_last = atomicAdd(&p.counters[seg], 1) == parts - 1;
-        if (s_last) p.counters[seg] = 0;  // ready for the next launch
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        kv4_join<D, W>(p, seg, (((long long)group0 + b) * p.heads + kvh) * p.group, (long long)p.heads * p.group, parts, reinterpret_cast<float*>(smem));
-      }
-    }
-    __syncthreads();  // the rings and the sums are free again
-
-    u = start = behind;
-    ++b;
+    __syncwarp();  // the ring is free
   }
 }
 
 template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long room, long long max_len, cudaStream_t st) {
   constexpr int bytes = W * Kv4Tile<D>::WARP + Kv4Tile<D>::QUERY;
-  static_assert(Kv4Tile<D>::RING >= 8 * D * 4, "a warp's ring holds its sums");
+  static_assert(Kv4Tile<D>::SPACE >= 4 * D * 4 && Kv4Tile<D>::SPACE >= 32 * 32, "a warp's space holds four heads of its sums");
   if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
   if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
   const long long most = p.batch * ((max_len - 1) / (32 * W) + 1);  // units, if no request is longer
