@@ -222,21 +222,6 @@ struct Kv4Attn {
 };
 
 template <int N> struct Words { uint32_t w[N]; };
-template <int N> struct Pairs { Pair p[N]; };
-template <int N> __device__ __forceinline__ Pairs<N> lds_pairs(const Pair* from) {
-  Pairs<N> r;
-  if constexpr (N == 1) {
-    const float2 v = *reinterpret_cast<const float2*>(from);
-    r.p[0] = {v.x, v.y};
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float4 v = *reinterpret_cast<const float4*>(from + i);
-      r.p[i] = {v.x, v.y}, r.p[i + 1] = {v.z, v.w};
-    }
-  }
-  return r;
-}
 template <int N> __device__ __forceinline__ Words<N> lds_words(const uint8_t* p) {
   Words<N> r;
   if constexpr (N == 1) r.w[0] = *reinterpret_cast<const uint32_t*>(p);
@@ -244,11 +229,30 @@ template <int N> __device__ __forceinline__ Words<N> lds_words(const uint8_t* p)
   else { const uint4 v = *reinterpret_cast<const uint4*>(p); r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w; }
   return r;
 }
+template <int N> struct Floats { float f[N]; };
+template <int N> __device__ __forceinline__ Floats<N> lds_floats(const float* p) {
+  const Words<N> w = lds_words<N>(reinterpret_cast<const uint8_t*>(p));
+  Floats<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.f[i] = __uint_as_float(w.w[i]);
+  return r;
+}
+template <int N> __device__ __forceinline__ void sts_floats(float* p, const Floats<N>& v) {
+  if constexpr (N == 1) *p = v.f[0];
+  else if constexpr (N == 2) *reinterpret_cast<float2*>(p) = make_float2(v.f[0], v.f[1]);
+  else *reinterpret_cast<float4*>(p) = make_float4(v.f[0], v.f[1], v.f[2], v.f[3]);
+}
+// An 8 x 8 matrix of 16-bit numbers, row gid and columns 2 tig, 2 tig + 1 to a lane, turned round.
+__device__ __forceinline__ uint32_t transpose(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
 template <int D> struct Kv4Tile {  // a tile of 32 keys in shared memory
   static constexpr int NG = D / 32, KEYS = 32, CODES = KEYS * D / 2, META = KEYS * NG * 4;
   static constexpr int K = 0, V = CODES, KM = 2 * CODES, VM = 2 * CODES + META, BYTES = 2 * (CODES + META);
-  static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4, RING = STAGES * BYTES, QUERY = 512 * (2 * NG + 2 * (NG < 4 ? 1 : NG / 4)), STEPS = 3 * 16 * NG * 8;
+  static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4, RING = STAGES * BYTES, QUERY = 512 * (NG + (NG < 4 ? 1 : NG / 4)), STEPS = 2 * KEYS * NG * 4;
   // behind a warp's ring: a tile's steps, or four heads of its sums when they meet those of the other warps
   static constexpr int SPACE = STEPS > 16 * D ? (STEPS > 1024 ? STEPS : 1024) : (16 * D > 1024 ? 16 * D : 1024);
   static constexpr int WARP = RING + SPACE;  // bytes of a warp; the query's are the CTA's
@@ -337,14 +341,11 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   auto same = [](int x) -> int { return __shfl_sync(0xffffffffu, x, 0); };
   const int warp = same(threadIdx.x >> 5), lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   uint8_t* ring = smem + warp * T::WARP;
-  // a tile's steps in fp32 as pairs of the two keys that a lane has in a block: [block 4][tig 4][group]; the group's place
-  // is turned by the block's number so that the 32 lanes, a key each, write without meeting in a bank
-  Pair* k_step = reinterpret_cast<Pair*>(ring + T::RING);
-  float* space = reinterpret_cast<float*>(ring + T::RING);
-  Pair *v_step = k_step + 16 * NG, *v_low = v_step + 16 * NG;
-  // the query as operand A, a register quad of each lane at a time: two steps of every group, two of (sum q, -8 sum q)
+  // a tile's steps (times a power of two) and lows of the values in fp32, [key][group]
+  float *v_step = reinterpret_cast<float*>(ring + T::RING), *v_low = v_step + 32 * NG;
+  float* space = v_step;
+  // the query as operand B, a lane's registers at a time: two steps of every group, then (sum q, -8 sum q) in three parts
   uint4* q_frag = reinterpret_cast<uint4*>(smem + W * T::WARP);
-  constexpr int TURN = (NG < 4 ? NG : 4) - 1;
 
   // a length beyond the table row is cut to the row, a row outside the table attends to nothing
   auto length = [&](int b) -> int {
@@ -481,12 +482,12 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
     cp_commit();
   };
 
-  float back = 0.f;  // undoes the query's power of two
-  // o: numbers 32 g + 4 gid + 2 i (+ 1: elements 2 and 3) of heads 2 tig and 2 tig + 1; z: sum p lo of head gid
-  float o[NG][2][4], mx = -INFINITY;
-  Pair z[NG], sum = {0.f, 0.f};
-  const int key_row = (gid & 1) ? ((gid >> 1) ^ 1) + 4 : gid >> 1;  // row of a block of 8 keys that column gid stands for
-  const int row_e[2] = {tig, (tig ^ 1) + 4};                        // rows of columns 2 tig and 2 tig + 1
+  // Of everything a lane has heads 2 tig and 2 tig + 1, as pairs.  back undoes the query's power of two; o: numbers 32 g +
+  // 4 gid + 2 i (+ 1: elements 2 and 3); sum, z: sums of p and p lo over this lane's keys.
+  float o[NG][2][4];
+  Pair back{}, mx{}, z[NG], sum{};
+  const int key_row = (gid & 1) ? ((gid >> 1) ^ 1) + 4 : gid >> 1;  // the key that row gid of a block of 8 stands for
+  const int row_e[2] = {tig, (tig ^ 1) + 4};                        // those of rows 2 tig and 2 tig + 1
   bool began = false, going = false;  // going: a request (cur) is in hand, its tiles are done; began: it began in this CTA
   if (u < u_end) enter(next, b, start);
   for (;;) {
@@ -502,18 +503,21 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       // ---- the warps' sums meet, four heads at a time
       const int seg = cur.b * p.heads + kvh;
       const bool whole = began && cur.behind <= u_end;
-      float l = sum.x + sum.y;
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (tig == 0) s_ml[warp][gid][0] = mx, s_ml[warp][gid][1] = l;
+      auto over_keys = [](Pair v) -> Pair {
+#pragma unroll
+        for (int i = 4; i < 32; i <<= 1) v.x += __shfl_xor_sync(0xffffffffu, v.x, i), v.y += __shfl_xor_sync(0xffffffffu, v.y, i);
+        return v;
+      };
+      const Pair l = over_keys(sum);
+      if (gid == 0) {
+        s_ml[warp][2 * tig][0] = mx.x, s_ml[warp][2 * tig][1] = l.x;
+        s_ml[warp][2 * tig + 1][0] = mx.y, s_ml[warp][2 * tig + 1][1] = l.y;
+      }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float zz = z[g].x + z[g].y;
-        zz += __shfl_xor_sync(0xffffffffu, zz, 1);
-        zz += __shfl_xor_sync(0xffffffffu, zz, 2);
-        const float z0 = __shfl_sync(0xffffffffu, zz, 8 * tig), z1 = __shfl_sync(0xffffffffu, zz, 8 * tig + 4);
+        const Pair zz = over_keys(z[g]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) o[g][i][0] += z0, o[g][i][1] += z1, o[g][i][2] += z0, o[g][i][3] += z1;
+        for (int i = 0; i < 2; ++i) o[g][i][0] += zz.x, o[g][i][1] += zz.y, o[g][i][2] += zz.x, o[g][i][3] += zz.y;
       }
 #pragma unroll 1
       for (int h0 = 0; h0 < p.group; h0 += 4) {
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
     began = u <= next.start;
     cur = next;
     going = true;
-    // ---- the query as operand A: row gid = head, numbers 32 w + 8 tig + (0 4 | 1 5 | 2 6 | 3 7) as pairs
+    // ---- the query as operand B: column gid = head, numbers 32 w + 8 tig + (0 4 | 1 5 | 2 6 | 3 7) as pairs
     {
       float x[NG][8], big = 0.f;
       const bool on = gid < p.group;
@@ -586,7 +590,8 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
       const int e = min(126, 140 - (int)(__float_as_uint(big) >> 23));
       const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-      back = __uint_as_float((uint32_t)(127 - e) << 23);
+      const float undo = __uint_as_float((uint32_t)(127 - e) << 23);
+      back = {__shfl_sync(0xffffffffu, undo, 8 * tig), __shfl_sync(0xffffffffu, undo, 8 * tig + 4)};
       float sums[NG];
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
@@ -598,8 +603,8 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         sums[w] = t * p.scale_log2;
         const float odd = up * 0.0625f;
         if (w % W != warp) continue;  // every warp has all of them, each brings its share
-        q_frag[(2 * w) * 32 + lane] = make_uint4(half2_bits(x[w][0] * up, x[w][4] * up), 0u, half2_bits(x[w][1] * odd, x[w][5] * odd), 0u);
-        q_frag[(2 * w + 1) * 32 + lane] = make_uint4(half2_bits(x[w][2] * up, x[w][6] * up), 0u, half2_bits(x[w][3] * odd, x[w][7] * odd), 0u);
+        q_frag[w * 32 + lane] = make_uint4(half2_bits(x[w][0] * up, x[w][4] * up), half2_bits(x[w][1] * odd, x[w][5] * odd),
+                                           half2_bits(x[w][2] * up, x[w][6] * up), half2_bits(x[w][3] * odd, x[w][7] * odd));
       }
 #pragma unroll
       for (int h = 0; h < BATCHES; ++h) {  // lane tig: (sum, -8 sum) of group 4 h + tig, in three parts
@@ -614,11 +619,10 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
           t -= part;
         }
         if (warp != W - 1) continue;
-        q_frag[(2 * NG + 2 * h) * 32 + lane] = make_uint4(parts[0], 0u, parts[1], 0u);
-        q_frag[(2 * NG + 2 * h + 1) * 32 + lane] = make_uint4(parts[2], 0u, 0u, 0u);
+        q_frag[(NG + h) * 32 + lane] = make_uint4(parts[0], parts[1], parts[2], 0u);
       }
     }
-    mx = -INFINITY, sum = {0.f, 0.f};
+    mx = {-INFINITY, -INFINITY}, sum = {0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       z[g] = {0.f, 0.f};
@@ -633,101 +637,106 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       const uint8_t* tile = ring + t * T::BYTES;
       const uint32_t mask = same(s_mask[warp][t]);
       if (mask == 0) continue;
-      // ---- steps: lane = key
+      // ---- steps of the values: lane = key
       float down;
       {
-        const int t = (lane & 4) ? (lane & 3) ^ 1 : lane & 3, n = lane >> 3;  // key row of (tig t, 0 or 1) of block n
-        float* at = reinterpret_cast<float*>(k_step + (4 * n + t) * NG) + ((lane >> 2) & 1);
         uint32_t largest = 0;
         Words<NB> v[BATCHES];
 #pragma unroll
         for (int h = 0; h < BATCHES; ++h) {
-          const Words<NB> k = lds_words<NB>(tile + T::KM + (lane * NG + h * NB) * 4);
           v[h] = lds_words<NB>(tile + T::VM + (lane * NG + h * NB) * 4);
 #pragma unroll
-          for (int w = 0; w < NB; ++w) {
-            at[2 * (h * NB + (w ^ (n & TURN)))] = high_bf16(k.w[w]);
-            largest = max(largest, v[h].w[w]);
-          }
+          for (int w = 0; w < NB; ++w) largest = max(largest, v[h].w[w]);
         }
-        // the power of two that puts the largest step of the values' tile into [2^14, 2^15)
+        // the power of two that puts the tile's largest step into [2^14, 2^15)
         largest = __reduce_max_sync(0xffffffffu, largest);
         const uint32_t ex = min(254u, 268u - min(254u, (largest >> 23) & 0xffu));
         const float up = __uint_as_float(ex << 23);
         down = __uint_as_float((278u - ex) << 23);  // 2^24 / up
 #pragma unroll
-        for (int h = 0; h < BATCHES; ++h)
+        for (int h = 0; h < BATCHES; ++h) {
+          Floats<NB> step, low;
 #pragma unroll
           for (int w = 0; w < NB; ++w) {
-            const float step = high_bf16(v[h].w[w]);
-            const int i = 2 * (h * NB + (w ^ (n & TURN)));
-            at[32 * NG + i] = step * up;
-            at[64 * NG + i] = fmaf(-8.f, step, low_bf16(v[h].w[w]));
+            step.f[w] = high_bf16(v[h].w[w]);
+            low.f[w] = fmaf(-8.f, step.f[w], low_bf16(v[h].w[w]));
+            step.f[w] *= up;
           }
+          sts_floats<NB>(v_step + lane * NG + h * NB, step);
+          sts_floats<NB>(v_low + lane * NG + h * NB, low);
+        }
         __syncwarp();
       }
-      // ---- logits of 4 blocks of 8 keys: this lane's head is gid, its keys row_e[0] and row_e[1] of each block
+      // ---- logits: keys are the rows of A (blocks 2 j and 2 j + 1 of 8), this lane has key key_row of each block
       const float none[4] = {0.f, 0.f, 0.f, 0.f};
-      Pair s[4];
-      Pair acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+      Pair s[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+      float term[2][4];
 #pragma unroll
-      for (int w = 0; w < NG; ++w) {
-        const uint4 q0 = q_frag[(2 * w) * 32 + lane], q1 = q_frag[(2 * w + 1) * 32 + lane];
+      for (int h = 0; h < BATCHES; ++h) {
+        Words<NB> codes[4], meta[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const int r = 8 * n + key_row;
-          const uint8_t* at = NG >= 4 ? tile + T::K + r * (D / 2) + (((4 * (w / 4) + tig) ^ T::swap(r)) * 16) + (w % 4) * 4 : tile + T::K + r * (D / 2) + tig * NG * 4 + w * 4;
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(at), y = x >> 8;
-          const Pair step = k_step[(4 * n + tig) * NG + (w & ~TURN) + ((w & TURN) ^ (n & TURN))];
-          float part[4];
-          mma_f16(part, q0, x & 0x000f000fu, x & 0x00f000f0u, none);
-          mma_f16(part, q1, y & 0x000f000fu, y & 0x00f000f0u, part);
-          acc[n] = fma2({part[0], part[1]}, step, acc[n]);
+          if constexpr (NG >= 4) codes[n] = lds_words<NB>(tile + T::K + r * (D / 2) + (((4 * h + tig) ^ T::swap(r)) * 16));
+          else codes[n] = lds_words<NB>(tile + T::K + r * (D / 2) + tig * NB * 4);
+          meta[n] = lds_words<NB>(tile + T::KM + (r * NG + h * NB) * 4);
+        }
+#pragma unroll
+        for (int w = 0; w < NB; ++w) {
+          const uint4 q = q_frag[(h * NB + w) * 32 + lane];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x0 = codes[2 * j].w[w], x1 = codes[2 * j + 1].w[w], y0 = x0 >> 8, y1 = x1 >> 8;
+            float part[4];
+            mma_f16(part, make_uint4(x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u), q.x, q.y, none);
+            mma_f16(part, make_uint4(y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u), q.z, q.w, part);
+            const float s0 = high_bf16(meta[2 * j].w[w]), s1 = high_bf16(meta[2 * j + 1].w[w]);
+            s[2 * j].x = fmaf(part[0], s0, s[2 * j].x), s[2 * j].y = fmaf(part[1], s0, s[2 * j].y);
+            s[2 * j + 1].x = fmaf(part[2], s1, s[2 * j + 1].x), s[2 * j + 1].y = fmaf(part[3], s1, s[2 * j + 1].y);
+          }
+        }
+        const uint4 q = q_frag[(NG + h) * 32 + lane];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t word[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            word[i] = tig < NB ? *reinterpret_cast<const uint32_t*>(tile + T::KM + ((16 * j + 8 * i + key_row) * NG + h * NB + (tig < NB ? tig : 0)) * 4) : 0u;
+          const uint4 a = make_uint4(word[0], word[1], word[0], word[1]);
+          if (h == 0) mma_bf16(term[j], a, q.x, q.y, none);
+          else mma_bf16(term[j], a, q.x, q.y, term[j]);
+          mma_bf16(term[j], a, q.z, 0u, term[j]);
         }
       }
-      float term[4][4];
 #pragma unroll
-      for (int h = 0; h < BATCHES; ++h) {
-        const uint4 q0 = q_frag[(2 * NG + 2 * h) * 32 + lane], q1 = q_frag[(2 * NG + 2 * h + 1) * 32 + lane];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const uint32_t word = tig < NB ? *reinterpret_cast<const uint32_t*>(tile + T::KM + ((8 * n + key_row) * NG + h * NB + (tig < NB ? tig : 0)) * 4) : 0u;
-          if (h == 0) mma_bf16(term[n], q0, word, word, none);
-          else mma_bf16(term[n], q0, word, word, term[n]);
-          mma_bf16(term[n], q1, word, 0u, term[n]);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) s[n] = fma2(mul2(acc[n], {back, back}), {p.scale_log2 * 0x1p24f, p.scale_log2 * 0x1p24f}, {term[n][0], term[n][1]});
+      for (int n = 0; n < 4; ++n)
+        s[n] = fma2(mul2(s[n], back), {p.scale_log2 * 0x1p24f, p.scale_log2 * 0x1p24f}, {term[n >> 1][2 * (n & 1)], term[n >> 1][2 * (n & 1) + 1]});
       if (mask != 0xffffffffu) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          if (!((mask >> (8 * n + row_e[0])) & 1)) s[n].x = -INFINITY;
-          if (!((mask >> (8 * n + row_e[1])) & 1)) s[n].y = -INFINITY;
-        }
+        for (int n = 0; n < 4; ++n)
+          if (!((mask >> (8 * n + key_row)) & 1)) s[n] = {-INFINITY, -INFINITY};
       }
       // ---- softmax of the tile
-      float top = mx;
+      Pair top = mx;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) top = fmaxf(top, fmaxf(s[n].x, s[n].y));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float zero = top == -INFINITY ? 0.f : top;
-      if (__any_sync(0xffffffffu, top != mx)) {
-        const float alpha = exp2f(mx - zero);
-        const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * tig), a1 = __shfl_sync(0xffffffffu, alpha, 8 * tig + 4);
-        sum = mul2(sum, {alpha, alpha});
+      for (int n = 0; n < 4; ++n) top.x = fmaxf(top.x, s[n].x), top.y = fmaxf(top.y, s[n].y);
+#pragma unroll
+      for (int i = 4; i < 32; i <<= 1) top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, i)), top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, i));
+      const Pair zero = {top.x == -INFINITY ? 0.f : top.x, top.y == -INFINITY ? 0.f : top.y};
+      if (__any_sync(0xffffffffu, top.x != mx.x || top.y != mx.y)) {
+        const Pair alpha = {exp2f(mx.x - zero.x), exp2f(mx.y - zero.y)};
+        sum = mul2(sum, alpha);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          z[g] = mul2(z[g], {alpha, alpha});
+          z[g] = mul2(z[g], alpha);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) o[g][t][0] *= a0, o[g][t][1] *= a1, o[g][t][2] *= a0, o[g][t][3] *= a1;
+          for (int i = 0; i < 2; ++i) o[g][i][0] *= alpha.x, o[g][i][1] *= alpha.y, o[g][i][2] *= alpha.x, o[g][i][3] *= alpha.y;
         }
         mx = top;
       }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        s[n].x = exp2f(s[n].x - zero), s[n].y = exp2f(s[n].y - zero);
+        s[n].x = exp2f(s[n].x - zero.x), s[n].y = exp2f(s[n].y - zero.y);
         sum = add2(sum, s[n]);
       }
       // ---- sum p lo, and sum (p s) c with p s in fp16; PB groups at a time
@@ -737,15 +746,11 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
         uint32_t codes[4][2], pb[4][PB];  // codes: a lane's numbers of two groups (D = 32: of one, a half word)
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          // the groups' place is turned by n: the pair of groups 2 h, 2 h + 1 lies at (2 h) ^ (n & 2) and is swapped by n & 1
-          const int at = (4 * n + tig) * NG + (h * PB ^ (n & TURN & ~(PB - 1)));
-          const Pairs<PB> step = lds_pairs<PB>(v_step + at), low = lds_pairs<PB>(v_low + at);
+          const Floats<PB> step = lds_floats<PB>(v_step + (8 * n + key_row) * NG + h * PB), low = lds_floats<PB>(v_low + (8 * n + key_row) * NG + h * PB);
 #pragma unroll
           for (int g = 0; g < PB; ++g) {
-            const int from = g ^ (n & TURN & (PB - 1));
-            const Pair ps = mul2(s[n], step.p[from]);
-            pb[n][g] = half2_bits(ps.x, ps.y);
-            z[h * PB + g] = fma2(s[n], low.p[from], z[h * PB + g]);
+            pb[n][g] = transpose(half2_bits(s[n].x * step.f[g], s[n].y * step.f[g]));
+            z[h * PB + g].x = fmaf(s[n].x, low.f[g], z[h * PB + g].x), z[h * PB + g].y = fmaf(s[n].y, low.f[g], z[h * PB + g].y);
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
