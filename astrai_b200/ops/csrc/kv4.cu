@@ -252,7 +252,7 @@ __device__ __forceinline__ uint32_t transpose(uint32_t v) {
 template <int D> struct Kv4Tile {  // a tile of 32 keys in shared memory
   static constexpr int NG = D / 32, KEYS = 32, CODES = KEYS * D / 2, META = KEYS * NG * 4;
   static constexpr int K = 0, V = CODES, KM = 2 * CODES, VM = 2 * CODES + META, BYTES = 2 * (CODES + META);
-  static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4, RING = STAGES * BYTES, QUERY = 512 * (NG + (NG < 4 ? 1 : NG / 4)), STEPS = 2 * KEYS * NG * 4;
+  static constexpr int STAGES = D == 256 ? 2 : 3, RING = STAGES * BYTES, QUERY = 512 * (NG + (NG < 4 ? 1 : NG / 4)), STEPS = 2 * KEYS * NG * 4;
   // behind a warp's ring: a tile's steps, or four heads of its sums when they meet those of the other warps
   static constexpr int SPACE = STEPS > 16 * D ? (STEPS > 1024 ? STEPS : 1024) : (16 * D > 1024 ? 16 * D : 1024);
   static constexpr int WARP = RING + SPACE;  // bytes of a warp; the query's are the CTA's
@@ -325,15 +325,15 @@ template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& 
 // What beginning and ending a request costs, in turns, and how far a cut is moved to spare one (both: mixed lengths of 16 to
 // 4608 took 33 us with 1 turn, 35 with 2, 36 with 3; 128 requests of 100 tokens 14.5, 12.5 and 14.5).
 constexpr int KV4_SETUP = 1, KV4_TOL = 1;
-// W warps a CTA; `per_sm` CTAs fit an SM (168 registers a thread up to D = 128, 255 beyond)
-template <int D, int W> constexpr int kv4_per_sm() { return W == 12 ? 1 : D == 256 ? 2 : 3; }
+// W warps a CTA; `per_sm` CTAs fit an SM (128, 168 and 255 registers a thread for D up to 64, 128 and 256)
+template <int D, int W> constexpr int kv4_per_sm() { return W == 12 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
 
 template <int D, int W>
 __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(const Kv4Attn p) {
   using T = Kv4Tile<D>;
   constexpr int NG = T::NG, NB = NG < 4 ? NG : 4, BATCHES = NG / NB, STAGES = T::STAGES, UNIT = 32 * W;
   constexpr int SETUP = KV4_SETUP, TOL = KV4_TOL;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t s_mask[W][STAGES];
   __shared__ float s_ml[W][8][2];
   __shared__ int s_scan[W], s_found[2][2], s_last;
