@@ -2,6 +2,7 @@
 // Only this file sees torch headers; kernels live in torch-free .cu files (launchers.h).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -365,6 +366,7 @@ void paged_decode_append_(const Tensor& q, const Tensor& k_new, const Tensor& v_
 // ---- 4-bit KV cache ----
 struct Kv4Pools {
   int64_t slots, heads, dim;
+  at::Device device;
 };
 
 // codes uint8 [slots, heads, D / 2], meta bf16 [slots, heads, D / 32, 2], the same shapes for keys and values.
@@ -373,7 +375,7 @@ Kv4Pools kv4_check(const char* what, const Tensor& k_codes, const Tensor& k_meta
     TORCH_CHECK(t->is_cuda() && t->is_contiguous() && t->device() == k_codes.device(), what, ": the pools must be contiguous CUDA tensors of one device");
   TORCH_CHECK(k_codes.scalar_type() == at::kByte && v_codes.scalar_type() == at::kByte && k_codes.dim() == 3 && v_codes.sizes() == k_codes.sizes(),
               what, ": k_codes / v_codes must be uint8 [slots, heads, head_dim / 2]");
-  const Kv4Pools p{k_codes.size(0), k_codes.size(1), 2 * k_codes.size(2)};
+  const Kv4Pools p{k_codes.size(0), k_codes.size(1), 2 * k_codes.size(2), k_codes.device()};
   TORCH_CHECK(p.dim == 32 || p.dim == 64 || p.dim == 128 || p.dim == 256, what, ": head_dim must be 32, 64, 128 or 256, got ", p.dim);
   for (const Tensor* t : {&k_meta, &v_meta})
     TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 4 && t->size(0) == p.slots && t->size(1) == p.heads &&
@@ -396,7 +398,7 @@ void kv4_check_loc(const char* what, const Tensor& loc, const Tensor& pool) {
 // Rows that the kernels can read in place: unit inner stride, every row on a 16-byte boundary.
 Tensor kv4_rows(const Tensor& t) {
   const bool ok = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 void kv4_check_new(const char* what, const Tensor& k, const Tensor& v, const Tensor& pool, int64_t tokens, const Kv4Pools& p) {
@@ -419,11 +421,16 @@ void kv4_append_(const Tensor& k, const Tensor& v, Tensor& k_codes, Tensor& k_me
   TORCH_CHECK(rc == 0, "kv4_append_ launch failed with code ", rc);
 }
 
+// A result: bf16 [rows, heads, numbers], asked of the allocator itself (a dispatched empty is a fifth of a small call's time).
+Tensor kv4_rows_for(int64_t rows, int64_t heads, const Kv4Pools& p) {
+  return at::detail::empty_cuda({rows, heads, p.dim}, at::kBFloat16, p.device, c10::nullopt);
+}
+
 std::tuple<Tensor, Tensor> kv4_gather(const Tensor& k_codes, const Tensor& k_meta, const Tensor& v_codes, const Tensor& v_meta, const Tensor& loc) {
   const Kv4Pools p = kv4_check("kv4_gather", k_codes, k_meta, v_codes, v_meta);
   kv4_check_loc("kv4_gather", loc, k_codes);
   const c10::cuda::CUDAGuard guard(k_codes.device());
-  Tensor k = at::empty({loc.numel(), p.heads, p.dim}, k_meta.options()), v = at::empty_like(k);
+  Tensor k = kv4_rows_for(loc.numel(), p.heads, p), v = kv4_rows_for(loc.numel(), p.heads, p);
   count();
   const int rc = ab::kv4_gather(k_codes.data_ptr(), k_meta.data_ptr(), v_codes.data_ptr(), v_meta.data_ptr(), loc.data_ptr(),
                                 loc.scalar_type() == at::kLong, k.data_ptr(), v.data_ptr(), loc.numel(), (int)p.heads, (int)p.dim, p.slots, stream());
@@ -493,6 +500,18 @@ void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_co
                                 (int)req_to_token.size(1), (int)req_to_token.size(0), p.slots, (float)scale, (int)parts,
                                 max_len, stream());
   TORCH_CHECK(rc == 0, "kv4_decode launch failed with code ", rc);
+}
+
+Tensor kv4_decode(const Tensor& q, Tensor& k_codes, Tensor& k_meta, Tensor& v_codes, Tensor& v_meta, const Tensor& req_to_token,
+                  const Tensor& req_pool_indices, const Tensor& seq_lens, const std::optional<Tensor>& k_new, const std::optional<Tensor>& v_new,
+                  double scale, int64_t max_len, const std::optional<Tensor>& o_part, const std::optional<Tensor>& ml_part,
+                  const std::optional<Tensor>& counters) {
+  const Kv4Pools p = kv4_check("kv4_decode", k_codes, k_meta, v_codes, v_meta);
+  TORCH_CHECK(q.dim() == 3, "kv4_decode: q must be bf16 [batch, heads, ", p.dim, "] on the pools' device");
+  Tensor out = kv4_rows_for(q.size(0), q.size(1), p);
+  kv4_decode_(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new, scale, max_len, o_part, ml_part,
+              counters, out);
+  return out;
 }
 
 // Page dst[i] of every layer of every pool [layers, slots, ...] becomes a copy of page src[i].
@@ -1280,6 +1299,7 @@ TORCH_LIBRARY(astrai_b200, m) {
   m.def("flash_fwd(Tensor q, Tensor k, Tensor v, Tensor? cu_q, Tensor? cu_k, int batch, int sq, int sk, int max_q, bool causal, float scale) -> (Tensor, Tensor)", &flash_fwd);
   m.def("kv4_append_(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor loc) -> ()", &kv4_append_);
   m.def("kv4_gather(Tensor k_codes, Tensor k_meta, Tensor v_codes, Tensor v_meta, Tensor loc) -> (Tensor, Tensor)", &kv4_gather);
+  m.def("kv4_decode(Tensor q, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor req_to_token, Tensor req_pool_indices, Tensor seq_lens, Tensor? k_new, Tensor? v_new, float scale, int max_len, Tensor? o_part, Tensor? ml_part, Tensor? counters) -> Tensor", &kv4_decode);
   m.def("kv4_decode_(Tensor q, Tensor(a!) k_codes, Tensor(b!) k_meta, Tensor(c!) v_codes, Tensor(d!) v_meta, Tensor req_to_token, Tensor req_pool_indices, Tensor seq_lens, Tensor? k_new, Tensor? v_new, float scale, int max_len, Tensor? o_part, Tensor? ml_part, Tensor? counters, Tensor(e!) out) -> ()", &kv4_decode_);
   m.def("copy_pages_(Tensor(a!)[] pools, int[] src, int[] dst, int page_size) -> ()", &copy_pages_);
   m.def("flash_fwd_paged(Tensor q, Tensor k_pool, Tensor v_pool, Tensor cu_q, Tensor cu_k, Tensor table, Tensor rows, int page, int max_q, bool causal, float scale) -> Tensor", &flash_fwd_paged);

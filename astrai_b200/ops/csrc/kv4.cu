@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kv4.cuh"
 #include "launchers.h"
 
@@ -792,7 +794,14 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
 template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long room, long long max_len, cudaStream_t st) {
   constexpr int bytes = W * Kv4Tile<D>::WARP + Kv4Tile<D>::QUERY;
   static_assert(Kv4Tile<D>::SPACE >= 4 * D * 4 && Kv4Tile<D>::SPACE >= 32 * 32, "a warp's space holds four heads of its sums");
-  if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
+  static std::atomic<unsigned long long> ready{0};  // devices that have been told (a tenth of a small call's time)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -5;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
   const long long most = p.batch * ((max_len - 1) / (32 * W) + 1);  // units, if no request is longer
   long long groups = 148 * kv4_per_sm<D, W>() / p.heads;

@@ -141,9 +141,10 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
     see :func:`kv4_decode_workspace`; without one the call allocates its own scratch."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     if k_codes.is_cuda:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         o_part, ml_part, counters = workspace if workspace is not None else (None, None, None)
+        if out is None:
+            return _op("kv4_decode")(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new,
+                                     scale, max_len, o_part, ml_part, counters)
         _op("kv4_decode_")(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new, scale,
                            max_len, o_part, ml_part, counters, out)
         return out

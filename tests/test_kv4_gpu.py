@@ -80,6 +80,25 @@ def test_slots_outside_the_pool_and_strided_rows():
             assert torch.equal(got.cpu(), want)
 
 
+def test_contiguous_rows_and_queries_that_start_off_a_16_byte_boundary():
+    from astrai_b200 import ops
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        return flat[1:].view(t.shape).copy_(t)
+
+    k, v, q = _rows(5, 2, 64, seed=5), _rows(5, 2, 64, seed=6), _rows(1, 4, 64, seed=7)
+    loc = torch.arange(5, device="cuda")
+    table, row, lens = torch.arange(5, dtype=torch.int32, device="cuda")[None], torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor([5], device="cuda")
+    results = []
+    for put in (lambda t: t, shifted):
+        pools = _pools(6, 2, 64)
+        ops.kv4_append_(put(k), put(v), *pools, loc)
+        out = ops.kv4_decode(put(q), *pools, table, row, lens, k_new=put(k[:1].clone()), v_new=put(v[:1].clone()), max_len=5)
+        results.append((*pools, out))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 # ---------------------------------------------------------------------------------------------------------- attention
 def _case(lens, heads, kv_heads, dim, seed, page=4, spare=3):
     """Pools whose slots outside the requests' positions read as NaN, a table, queries and a step's rows."""
