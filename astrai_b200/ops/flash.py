@@ -75,8 +75,11 @@ def flash_attention_varlen(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
     d = q.shape[-1]
     scale = float(scale) if scale is not None else d ** -0.5
     batch = cu_seqlens_q.numel() - 1
-    return _FlashFn.apply(q, k, v, cu_seqlens_q.int(), cu_seqlens_k.int(), batch, 0, 0, int(max_q), int(max_k),
-                          bool(causal), scale)
+    cu_q, cu_k = cu_seqlens_q.int(), cu_seqlens_k.int()
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        # nothing to keep for a backward pass: serving's short prompts spend more time in Python than on the GPU
+        return torch.ops.astrai_b200.flash_fwd(_fix(q), _fix(k), _fix(v), cu_q, cu_k, batch, 0, 0, int(max_q), bool(causal), scale)[0]
+    return _FlashFn.apply(q, k, v, cu_q, cu_k, batch, 0, 0, int(max_q), int(max_k), bool(causal), scale)
 
 
 PAGED_PAGE_SIZES = (8, 16, 32, 64)

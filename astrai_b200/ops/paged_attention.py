@@ -27,9 +27,6 @@ from astrai_b200.ops.kv import KVCache
 
 
 def _append(k: Tensor, v: Tensor, cache: KVCache, layer_id: int):
-    if cache.four_bit:
-        kv4.kv4_append_(k, v, *cache.layer_pools(layer_id), cache.out_cache_loc.reshape(-1))
-        return
     kb, vb = cache.k_buffer[layer_id], cache.v_buffer[layer_id]
     loc = cache.out_cache_loc.reshape(-1)
     if k.is_cuda and k.dtype == torch.bfloat16 and kb.dtype == torch.bfloat16 and (kb.shape[1] * kb.shape[2]) % 8 == 0:
@@ -115,15 +112,19 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
             kv_cache.req_to_token, kv_cache.req_pool_indices, kv_cache.seq_lens, scale, splits, kv_cache.decode_o_part,
             kv_cache.decode_ml_part, kv_cache.decode_counters, out)
         return out
-    _append(k, v, kv_cache, layer_id)
+    pools = kv_cache.layer_pools(layer_id) if kv_cache.four_bit else None
+    if pools is not None:
+        kv4.kv4_append_(k, v, *pools, kv_cache.out_cache_loc.reshape(-1))
+    else:
+        _append(k, v, kv_cache, layer_id)
     q_lens, kv_lens = _lens(kv_cache)
     page = getattr(kv_cache, "page_size", 1) or 1
-    if kv_cache.four_bit:
+    if pools is not None:
         if (native_on and attn_mask is None and fwd == "prefill" and kv_cache.kv_gather_loc is not None
                 and kv_cache.qo_indptr is not None and q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in flash.SUPPORTED_HEAD_DIMS):
             # the prompt's own rows are read back with the cached ones: a token sees the same numbers of a key whether its
             # prompt ran in one chunk or several
-            kk, vv = kv4.kv4_gather(*kv_cache.layer_pools(layer_id), kv_cache.kv_gather_loc)
+            kk, vv = kv4.kv4_gather(*pools, kv_cache.kv_gather_loc)
             return flash.flash_attention_varlen(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens),
                                                 causal=True, scale=scale)
     elif (native_on and attn_mask is None and fwd == "prefill" and kv_cache.qo_indptr is not None and page in flash.PAGED_PAGE_SIZES
