@@ -282,7 +282,7 @@ def prefill(preset, ckpt, config_path, device, dtype, cache, kv_dtype, backend, 
                 if i >= 3:
                     times.append(time.perf_counter() - t0)
         best = min(times)
-        rows.append({"benchmark": "prefill", "model": name, "backend": sched.backend_name, "cache": cache, "batch": batch_size,
+        rows.append({"benchmark": "prefill", "model": name, "backend": sched.backend_name, "cache": cache, "kv_dtype": kv_dtype, "batch": batch_size,
                      "prompt_len": prompt_len, "tok_per_s": batch_size * prompt_len / best, "ms": best * 1e3})
         del sched
     _report(rows, "tok_per_s")
@@ -312,7 +312,7 @@ def decode(preset, ckpt, config_path, device, dtype, cache, kv_dtype, backend, c
             _sync(device)
             dt = time.perf_counter() - t0
         n = sum(len(o[0]) if isinstance(o, tuple) else len(o) for o in out)
-        rows.append({"benchmark": "decode", "model": name, "backend": sched.backend_name, "cache": cache, "cuda_graph": sched.cuda_graph_enabled,
+        rows.append({"benchmark": "decode", "model": name, "backend": sched.backend_name, "cache": cache, "kv_dtype": kv_dtype, "cuda_graph": sched.cuda_graph_enabled,
                      "batch": batch_size, "gen_len": gen_len, "tok_per_s": n / dt, "ms_per_step": dt * 1e3 / max(gen_len, 1)})
         del sched
     _report(rows, "tok_per_s")

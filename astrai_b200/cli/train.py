@@ -123,6 +123,7 @@ def build_train_config(o: Dict[str, Any]):
         start_method=o["start_method"], device_type=o["device_type"], val_split=o["val_split"], val_step=o["val_step"],
         neftune_alpha=o["neftune_alpha"], rollout_interval=o["rollout_interval"], rollout_temperature=o["rollout_temperature"],
         rollout_top_k=o["rollout_top_k"], rollout_top_p=o["rollout_top_p"], rollout_max_tokens=o["rollout_max_tokens"],
+        rollout_share_prompts=o.get("rollout_share_prompts", False),
         executor_kwargs=executor_kwargs, strategy_kwargs=strategy_kwargs(o),
     ), total_steps
 
@@ -261,6 +262,8 @@ def plan(o: Dict[str, Any]) -> Dict[str, Any]:
 @click.option("--rollout_top_k", type=int, default=0, help="online_*: top-k (0 = off).")
 @click.option("--rollout_top_p", type=float, default=0.9, help="online_*: top-p.")
 @click.option("--rollout_max_tokens", type=int, default=1024, help="online_*: longest sampled response.")
+@click.option("--rollout_share_prompts/--no-rollout_share_prompts", default=False,
+              help="online_*: prefill each prompt once and fork its KV cache for the group's other responses.")
 @click.pass_context
 def train_command(ctx: click.Context, config: Optional[str], **opts):
     """Train a decoder LM (seq / sft / dpo / grpo, offline or with online rollouts)."""

@@ -78,6 +78,7 @@ class TrainConfig(BaseConfig):
     rollout_top_k: int = 0
     rollout_top_p: float = 0.9
     rollout_max_tokens: int = 1024
+    rollout_share_prompts: bool = False
     reward_model_fn: Optional[Callable] = None
     executor_kwargs: Dict[str, Any] = field(default_factory=dict)
     strategy_kwargs: Dict[str, Any] = field(default_factory=dict)

@@ -291,7 +291,8 @@ class ContiguousStrategy(AllocationStrategy):
         return True
 
     def fork(self, src, dst, length, copy):
-        copy([src.req_idx], [dst.req_idx])  # a row of the contiguous layout is one page
+        if length:
+            copy([src.req_idx], [dst.req_idx])  # a row of the contiguous layout is one page
         return True
 
     def write_indices(self, state, prompt_ids):

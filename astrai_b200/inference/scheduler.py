@@ -52,6 +52,8 @@ class InferenceScheduler:
         p = next(model.parameters())
         self.device = torch.device(device) if device is not None else p.device
         self.dtype = dtype or p.dtype
+        if cache is not None and kv_dtype not in ("auto", getattr(cache, "kv_dtype", "auto")):
+            raise ValueError(f"kv_dtype {kv_dtype!r} was asked for, but the cache that was given holds {getattr(cache, 'kv_dtype', 'auto')!r}")
         self._cache = cache if cache is not None else PagePool.for_model(
             cfg, max_batch_size, max_seq_len, self.device, self.dtype, page_size=page_size, n_tokens=kv_cache_tokens, paged=paged,
             kv_dtype=kv_dtype)

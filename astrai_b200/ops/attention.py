@@ -116,6 +116,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, kv_cache=None, layer_id: int = 0,
 
     own = backend.current_custom()
     if own is not None:  # a registered back end that computes attention itself
+        if getattr(kv_cache, "four_bit", False) and not own.reads_four_bit:
+            raise ValueError(f"{type(own).__name__} does not read a 4-bit KV cache (a back end that does sets reads_four_bit)")
         return own.forward(q, k, v, kv_cache, layer_id, attn_mask, is_causal, fwd)
     if fwd is None:
         return dense_attention(q, k, v, attn_mask, is_causal)

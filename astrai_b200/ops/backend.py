@@ -52,6 +52,8 @@ class AttentionBackend:
     """
 
     kind: Optional[ATTN_BACKEND] = None  # built-in back ends: the enum member they stand for
+    # whether the back end reads a 4-bit cache (``kv_cache.four_bit``: the buffers hold codes, see :mod:`astrai_b200.ops.kv4`)
+    reads_four_bit: bool = False
 
     def __enter__(self) -> "AttentionBackend":
         self._token = _current.set(self.kind if self.kind is not None else self)

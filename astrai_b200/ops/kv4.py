@@ -132,7 +132,7 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
 
     ``q [batch, heads, D]``; request ``i`` has ``seq_lens[i]`` positions (int64) whose slots are
     ``req_to_token[req_pool_indices[i], :seq_lens[i]]`` (int32).  ``k_new`` / ``v_new [batch, kv_heads, D]`` are stored
-    into the last position's slot first (when absent, the pool already holds them).  A request of length 0 gives zeros;
+    into the last position's slot first (when absent, the pool already holds them; two requests must not store into one slot).  A request of length 0 gives zeros;
     positions whose slot is outside the pool are left out.  The numbers of the cache enter unrounded, sums and softmax are
     fp32, the result is bf16.
 

@@ -278,6 +278,6 @@ class TrainContextBuilder:
                                        max_seq_len=getattr(inner.config, "max_position_embeddings", None))
         generator = RolloutGenerator(scheduler=scheduler, tokenizer=tokenizer, max_tokens=c.rollout_max_tokens,
                                      group_size=group, temperature=c.rollout_temperature, top_k=c.rollout_top_k,
-                                     top_p=c.rollout_top_p)
+                                     top_p=c.rollout_top_p, share_prompts=c.rollout_share_prompts)
         ctx.strategy.set_rollout_runner(RolloutRunner(generator=generator, reward_model=c.reward_model_fn(),
                                                       rollout_interval=c.rollout_interval))

@@ -317,3 +317,78 @@ def test_rollouts_can_share_prompts(model):
         gen = RolloutGenerator(_scheduler(model), Tok(), max_tokens=5, group_size=3, temperature=0.0, share_prompts=share)
         outs.append(gen.generate(batch))
     assert torch.equal(outs[0].responses, outs[1].responses) and torch.equal(outs[0].response_mask, outs[1].response_mask)
+
+
+def test_online_training_shares_prompts(tmp_path):
+    """The option reaches the scheduler: each prompt of a batch is asked for once, with a group of answers."""
+    from astrai_b200.config import TrainConfig
+    from astrai_b200.inference.scheduler import InferenceScheduler
+    from astrai_b200.trainer import Trainer
+    from helpers import build_tokenizer_dir
+    from test_online_training import Instructions, LongerIsBetter, _adamw, _model, collate
+
+    asked, plain = [], InferenceScheduler.run_batch
+
+    def run_batch(self, prompts, **kw):
+        asked.append((len(prompts), kw.get("samples_per_prompt", 1)))
+        return plain(self, prompts, **kw)
+
+    cfg = dict(strategy="online_grpo", model_fn=_model, dataset=Instructions(), optimizer_fn=_adamw, n_epoch=1, batch_per_device=2,
+               grad_accum_steps=1, ckpt_interval=100, random_seed=42, device_type="cpu", backend="gloo", nprocs=1, parallel_mode="none",
+               strategy_kwargs={"clip_eps": 0.2, "kl_coef": 0.01, "group_size": 3}, rollout_interval=1, rollout_max_tokens=4,
+               reward_model_fn=LongerIsBetter, collate_fn=collate, metrics=["loss"])
+    params = build_tokenizer_dir(str(tmp_path / "params"))
+    InferenceScheduler.run_batch = run_batch
+    try:
+        Trainer(TrainConfig(**cfg, ckpt_dir=str(tmp_path / "ck"), rollout_share_prompts=True)).train(param_path=params)
+    finally:
+        InferenceScheduler.run_batch = plain
+    assert asked and all(a == (2, 3) for a in asked)
+
+
+def test_back_ends_and_caches_that_do_not_fit_are_refused(model):
+    from astrai_b200.inference.cache import PagePool
+    from astrai_b200.ops import AttentionBackend, attn_backend
+
+    class Own(AttentionBackend):
+        def fwd_prefill(self, q, k, v, kv_cache, layer_id, attn_mask=None, is_causal=False):
+            from astrai_b200.ops.paged_attention import cached_attention
+
+            with attn_backend("torch_native"):
+                return cached_attention(q, k, v, kv_cache, layer_id, attn_mask, is_causal, "prefill")
+
+        fwd_decode = fwd_prefill
+
+    class Reads(Own):
+        reads_four_bit = True
+
+    prompt = [list(range(5, 14))]
+    want = _scheduler(model).run_batch(prompt, max_tokens=4, temperature=0.0)
+    with attn_backend(Own()):
+        with pytest.raises(ValueError, match="Own does not read a 4-bit"):
+            _scheduler(model).run_batch(prompt, max_tokens=4, temperature=0.0)
+        assert _scheduler(model, kv_dtype="auto").run_batch(prompt, max_tokens=4, temperature=0.0)[0]
+    with attn_backend(Reads()):
+        assert _scheduler(model).run_batch(prompt, max_tokens=4, temperature=0.0) == want
+    pool = PagePool.for_model(model.config, 8, 48, "cpu", torch.float32, page_size=4)
+    with pytest.raises(ValueError, match="'int4' was asked for"):
+        _scheduler(model, cache=pool)
+    four = PagePool.for_model(model.config, 8, 48, "cpu", torch.float32, page_size=4, kv_dtype="int4")
+    for kw in ({"kv_dtype": "auto"}, {}):  # the cache that was given decides
+        assert _scheduler(model, cache=four, **kw).run_batch(prompt, max_tokens=4, temperature=0.0) == want
+
+
+def test_commands_hand_the_options_on(tmp_path, monkeypatch):
+    from click.testing import CliRunner
+
+    from astrai_b200.cli import serve
+    from astrai_b200.cli.benchmark import benchmark as bench
+
+    got = {}
+    monkeypatch.setattr("astrai_b200.inference.network.app.run_server", lambda **kw: got.update(kw))
+    monkeypatch.setattr("astrai_b200.inference.run_server", lambda **kw: got.update(kw), raising=False)
+    res = CliRunner().invoke(serve.serve_command, ["--param_path", str(tmp_path), "--kv_dtype", "int4", "--device", "cpu"])
+    assert res.exit_code == 0, res.output
+    assert got["kv_dtype"] == "int4"
+    assert CliRunner().invoke(serve.serve_command, ["--param_path", str(tmp_path), "--kv_dtype", "int3"]).exit_code == 2
+    assert all(any(p.name == "kv_dtype" for p in bench.commands[c].params) for c in ("prefill", "decode", "serve"))
