@@ -473,11 +473,11 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       cp_async<PIECE>(to + T::VM, p.v_meta + (uint64_t)at_row + i * (PIECE / 4));
     }
   };
-  int ahead = 0, slot = -1;  // the next tile to copy, and its slots
+  int ahead = 0, slot = -1, slot_after = -1;  // the next tile to copy, its slots and those of the one behind it
   auto copy_next = [&](const Part& r, int stage) {
     if (ahead < r.key_end) {
       const int now = slot;
-      slot = slot_of(r, ahead + UNIT);
+      slot = slot_after, slot_after = slot_of(r, ahead + 2 * UNIT);
       issue(r, ahead, now, stage);
       ahead += UNIT;
     }
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
     const bool more = going ? cur.behind < u_end : u < u_end;
     if (more) {
       if (going) u = cur.behind, enter(next, cur.b + 1, cur.behind);
-      ahead = next.key, slot = slot_of(next, ahead);
+      ahead = next.key, slot = slot_of(next, ahead), slot_after = slot_of(next, ahead + UNIT);
 #pragma unroll 1
       for (int t = 0; t < STAGES - 1; ++t) copy_next(next, t);
     }
