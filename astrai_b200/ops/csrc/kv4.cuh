@@ -48,6 +48,13 @@ __device__ __forceinline__ uint32_t min_bf162(uint32_t a, uint32_t b) {  // of b
   return r;
 }
 
+// The two numbers, cut to 0 .. 15, before the codes that are there already.
+__device__ __forceinline__ uint32_t pack_codes(int high, int low, uint32_t behind) {
+  uint32_t r;
+  asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(high), "r"(low), "r"(behind));
+  return r;
+}
+
 // Eight numbers of a lane -> their eight codes (lowest number in the lowest half byte) and the (m, s) word of the group,
 // which four neighbouring lanes share.  Every lane of the warp takes part.
 __device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, uint32_t& meta) {
@@ -81,17 +88,20 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, u
   v.unpack(x);
   uint32_t word = 0;
 #pragma unroll
-  for (int j = 7; j >= 0; --j) {
-    const float y = sub_ieee(x[j], m);
-    const float big = fmaf(y, inv, 12582912.f);  // 1.5 2^23 + c': the whole number in the low bits
-    float c = big - 12582912.f;
-    const float rest = fma_ieee(-c, s, y);
-    const float most = __uint_as_float(__float_as_uint(half) - (__float_as_uint(big) & 1u));  // an odd c' may not have s / 2 left
-    if (fabsf(rest) > most) c += __uint_as_float((__float_as_uint(rest) & 0x80000000u) | 0x3f800000u);
-    c = fminf(fmaxf(c, -8.f), 7.f) + 8388616.f;  // 2^23 + c
-    word = word * 16u + __float_as_uint(c);
+  for (int j = 7; j >= 0; j -= 2) {
+    int code[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float y = sub_ieee(x[j - i], m);
+      float big = fmaf(y, inv, 12582912.f);  // 1.5 2^23 + c': the whole number in the low bits
+      const float rest = fma_ieee(12582912.f - big, s, y);
+      const float most = __uint_as_float(__float_as_uint(half) - (__float_as_uint(big) & 1u));  // an odd c' may not have s / 2 left
+      if (fabsf(rest) > most) big += __uint_as_float((__float_as_uint(rest) & 0x80000000u) | 0x3f800000u);
+      code[i] = (int)__float_as_uint(big) - (0x4b400000 - 8);
+    }
+    word = pack_codes(code[0], code[1], word);
   }
-  return word - 0xfb000000u;  // the share of the exponents: sum of 0x4b000000 16^j, as far as it fits
+  return word;
 }
 
 // One row per D / 8 lanes: lane `l` of the row brings its numbers 8 l .. 8 l + 7 (`src`), and the row goes to `codes` /
