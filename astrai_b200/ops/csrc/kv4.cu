@@ -12,7 +12,9 @@
 namespace ab {
 
 // ------------------------------------------------------------------------------------------------------- store rows
-// D / 8 lanes a row, a key row and a value row each.  A slot outside the pool is skipped.
+// D / 8 lanes a row, a key row and a value row each, both on their way before the first is worked on.  A slot outside the
+// pool is skipped.  Bound by its instructions, 420 a warp for 2 x 256 numbers: 8192 tokens of 8 heads of 128 numbers take
+// 16.6 us, of which 12 are issue slots, 6.7 the 44 MB that move; 16 tokens take 2 us (a launch).
 template <int D, typename Loc>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v,
                                                          uint8_t* __restrict__ k_codes, uint32_t* __restrict__ k_meta,
@@ -25,12 +27,15 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __nv_bfloat16* __
   const long long slot = r < rows ? (long long)loc[t] : -1;
   const bool live = slot >= 0 && slot < n_slots;
   const long long at = live ? slot * heads + h : 0;
-  kv4_store_row<D>(live, true, l, k + t * k_tok + h * k_head, k_codes + at * (D / 2), k_meta + at * (D / 32));
-  kv4_store_row<D>(live, false, l, v + t * v_tok + h * v_head, v_codes + at * (D / 2), v_meta + at * (D / 32));
+  const Vec8<__nv_bfloat16> kv = kv4_load_numbers(live, l, k + t * k_tok + h * k_head), vv = kv4_load_numbers(live, l, v + t * v_tok + h * v_head);
+  kv4_store_numbers<D>(live, true, l, kv, k_codes + at * (D / 2), k_meta + at * (D / 32));
+  kv4_store_numbers<D>(live, false, l, vv, v_codes + at * (D / 2), v_meta + at * (D / 32));
 }
 
 // -------------------------------------------------------------------------------------------------------- read rows
-// The reverse, as bf16 rows [tokens, heads, D].  A slot outside the pool reads as zeros.
+// The reverse, as bf16 rows [tokens, heads, D].  A slot outside the pool reads as zeros.  Bound by memory: 131072 tokens of
+// 8 heads of 128 numbers (705 MB) take 122 us, 5.8 TB/s (88% of a copy's rate).  The rows are written past the caches: they
+// would push out the codes of the next call.
 __device__ __forceinline__ uint4 kv4_numbers(uint32_t word, uint32_t ms) {
   const float m = __uint_as_float(ms << 16), s = __uint_as_float(ms & 0xffff0000u);
   float x[8];
@@ -157,6 +162,20 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
 // warp w takes every W-th tile of 32 keys, streams it through a ring of its own in shared memory (cp.async, no barrier
 // between warps), and the warps' sums meet at the end of the request.  What several groups share of a request is joined by
 // the one that finishes last.
+//
+// What it takes, and what bounds it.  16 requests of 65521 tokens, 16 query over 4 kv heads, D = 128 (671 MB of codes and
+// steps): 157 us, 4.3 TB/s, 65% of a copy's rate.  The loop without its copies takes 137 us, the copies without the
+// arithmetic 123 us.  The arithmetic waits more than it works: with three warps a scheduler (162 registers a thread) half
+// of the issue slots are taken, 43% of the integer pipe's, 33% of the shared memory's, 19% of the tensor pipe's (a tile
+// of 32 keys has a chain of products, a maximum over lanes, exponentials and products again).  Four warps a scheduler at
+// 128 registers spilled and took 190 us.  A launch begins with some 5 us of lengths, table, slots and first tiles and ends
+// with 3 to 4 us in which sums meet, and shorter work is bound by those: one request of 65521 tokens over 8 kv heads
+// 34.7 us (floor 12.8), 128 requests of 16 to 4608 tokens over 4 28.8 us (floor 11.8), 32 of 2049 to 8191 over 4 of 64
+// numbers 26.8 us (floor 7.0), 64 of 1000 over 4 of 256 numbers 34.5 us, one of 8192 over 4 12.4 us, 4 of 1 to 33 6.2 us.
+//
+// Keys are the rows of the logits' product and queries its columns: a lane then holds two keys' steps, and eight query heads
+// fill the columns (with queries as rows, half of them empty, the 16 requests took 177 us).  The products of the weights
+// take queries as columns too, so the weights are turned round in registers (movmatrix).
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
   if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -251,7 +270,9 @@ __device__ __forceinline__ uint32_t transpose(uint32_t v) {
   return r;
 }
 
-template <int D> struct Kv4Tile {  // a tile of 32 keys in shared memory
+// A tile of 32 keys in shared memory.  STAGES: tiles of a warp's ring; three, two where three do not fit (with two, D = 128,
+// 16 requests of 65521 tokens: 161 us instead of 158).
+template <int D> struct Kv4Tile {
   static constexpr int NG = D / 32, KEYS = 32, CODES = KEYS * D / 2, META = KEYS * NG * 4;
   static constexpr int K = 0, V = CODES, KM = 2 * CODES, VM = 2 * CODES + META, BYTES = 2 * (CODES + META);
   static constexpr int STAGES = D == 256 ? 2 : 3, RING = STAGES * BYTES, QUERY = 512 * (NG + (NG < 4 ? 1 : NG / 4)), STEPS = 2 * KEYS * NG * 4;
@@ -324,10 +345,12 @@ template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& 
   }
 }
 
-// What beginning and ending a request costs, in turns, and how far a cut is moved to spare one (both: mixed lengths of 16 to
-// 4608 took 33 us with 1 turn, 35 with 2, 36 with 3; 128 requests of 100 tokens 14.5, 12.5 and 14.5).
+// What beginning and ending a request costs, in turns, and how far a cut is moved to spare one (both: 128 mixed lengths of 16
+// to 4608 took 28.8 us with 1 turn, 30.9 with 2, 34.5 with 3; 128 requests of 100 tokens 13.2, 11.5 and 13.0; cuts that are
+// not moved: 30.8 and 13.0).
 constexpr int KV4_SETUP = 1, KV4_TOL = 1;
-// W warps a CTA; `per_sm` CTAs fit an SM (128, 168 and 255 registers a thread for D up to 64, 128 and 256)
+// W warps a CTA; `per_sm` CTAs fit an SM: 128, 168 and 255 registers a thread for D up to 64, 128 and 256 (D = 64, 16
+// requests of 65521 tokens: three CTAs 116 us, four 105; shared memory that does not begin on a 128-byte line: 137).
 template <int D, int W> constexpr int kv4_per_sm() { return W == 12 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
 
 template <int D, int W>
@@ -813,7 +836,9 @@ template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long r
   return cudaGetLastError() == cudaSuccess ? 0 : -5;
 }
 
-// Where the workspace has fewer parts than a wave of CTAs would make (few long requests), each is made by more warps.
+// Where the workspace has fewer parts than a wave of CTAs would make (few long requests), each is made by more warps: one
+// request of 65521 tokens over 8 kv heads, 32 parts, takes 34.7 us with 12 warps a CTA and 37.3 with 4.  Elsewhere a cut
+// every 128 keys divides the work better than one every 384: 128 mixed requests 28.8 us with 4 warps, 39.1 with 12.
 template <int D> static int kv4_attn_pick(const Kv4Attn& p, int parts, long long max_len, cudaStream_t st) {
   const long long room = (long long)p.batch * (parts - 1) + 1;
   if constexpr (D <= 128) {
@@ -846,7 +871,8 @@ int kv4_decode(const void* q, void* k_codes, void* k_meta, void* v_codes, void* 
 
 // ------------------------------------------------------------------------------------------------------- copy pages
 // Page dst[i] of every layer of every pool becomes a copy of page src[i].  The page numbers travel in the launch's
-// parameters, so the call keeps no buffer alive and can be captured into a graph as it stands.
+// parameters, so the call keeps no buffer alive and can be captured into a graph as it stands.  Bound by memory: 192 pages
+// of 16 tokens in 32 layers of 8 heads of 128 numbers in 4 bits (252 MB read and written) take 40 us, 96% of a copy's rate.
 template <typename Unit>
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ PageCopies c) {
   const int pool = blockIdx.z, layer = blockIdx.y, pair = blockIdx.x;

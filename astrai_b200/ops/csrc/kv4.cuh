@@ -104,14 +104,11 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Vec8<__nv_bfloat16>& v, u
   return word;
 }
 
-// One row per D / 8 lanes: lane `l` of the row brings its numbers 8 l .. 8 l + 7 (`src`), and the row goes to `codes` /
-// `meta`.  Every lane of the warp takes part; a lane with `live` false stores nothing (and its `src` is not read).
+// One row per D / 8 lanes: lane `l` of the row brings its numbers 8 l .. 8 l + 7, and the row goes to `codes` / `meta`.
+// Every lane of the warp takes part; a lane with `live` false stores nothing.
 template <int D>
-__device__ __forceinline__ void kv4_store_row(bool live, bool key, int l, const __nv_bfloat16* src, uint8_t* codes, uint32_t* meta) {
+__device__ __forceinline__ void kv4_store_numbers(bool live, bool key, int l, const Vec8<__nv_bfloat16>& v, uint8_t* codes, uint32_t* meta) {
   constexpr int NG = D / 32;
-  Vec8<__nv_bfloat16> v;
-  v.raw = make_uint4(0, 0, 0, 0);
-  if (live) v.load(src + 8 * l);
   uint32_t ms;
   const uint32_t word = kv4_quantise(v, ms);
   // a value row's words are made of two half words that two lanes may hold
@@ -127,6 +124,18 @@ __device__ __forceinline__ void kv4_store_row(bool live, bool key, int l, const 
   if (key) reinterpret_cast<uint32_t*>(codes)[kv4_key_word<D>(l >> 2, l & 3)] = word;
   else reinterpret_cast<uint32_t*>(codes)[l] = out;
   if ((l & 3) == 0) meta[l >> 2] = ms;
+}
+
+// The same from memory: `src` is the row, not read where `live` is false.
+__device__ __forceinline__ Vec8<__nv_bfloat16> kv4_load_numbers(bool live, int l, const __nv_bfloat16* src) {
+  Vec8<__nv_bfloat16> v;
+  v.raw = make_uint4(0, 0, 0, 0);
+  if (live) v.load(src + 8 * l);
+  return v;
+}
+template <int D>
+__device__ __forceinline__ void kv4_store_row(bool live, bool key, int l, const __nv_bfloat16* src, uint8_t* codes, uint32_t* meta) {
+  kv4_store_numbers<D>(live, key, l, kv4_load_numbers(live, l, src), codes, meta);
 }
 
 }  // namespace ab
