@@ -1,4 +1,4 @@
-"""Kernel timing harness: ``python -m astrai_b200.ops.bench_kernels {gemm,skinny,flash,fp8,quant,sample,decode}``.
+"""Kernel timing harness: ``python -m astrai_b200.ops.bench_kernels {gemm,skinny,flash,fp8,quant,sample,decode,kv4}``.
 
 CUDA events on the launching stream, 3 warm-ups, median of N timed launches, a 256 MB buffer written between timed
 launches to flush the 126 MB L2.  Library kernels (cuBLAS through ``torch.matmul``, cuDNN / flash through SDPA) are
@@ -196,8 +196,61 @@ def bench_decode():
         print(f"  B={b:3d} ctx={ctx:5d} {hq}q/{hkv}kv D{d} splits={splits:2d}: {ms * 1e3:7.1f} us  {gb / ms:6.0f} GB/s")
 
 
+def bench_kv4():
+    """The 4-bit KV cache: decode attention on the codes next to the bf16 pool's kernel, rows in and out, page copies."""
+    from astrai_b200 import ops
+    from astrai_b200.ops import native
+
+    native.require()
+    t = _timer()
+    op = torch.ops.astrai_b200
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def pools(slots, heads, d, layers=None):
+        lead = (slots, heads) if layers is None else (layers, slots, heads)
+        return [x for _ in "kv" for x in (torch.zeros(*lead, d // 2, dtype=torch.uint8, device="cuda"),
+                                          torch.zeros(*lead, d // 32, 2, dtype=torch.bfloat16, device="cuda"))]
+
+    print("decode attention over 16-token pages in random order (us, GB/s of the cache): 4 bits | bf16 pool; heads q/kv, head dim")
+    for lens, hq, hkv, d in [([1, 12, 20, 33], 4, 2, 64), ([65521], 32, 8, 128), ([16 + 36 * i for i in range(128)], 16, 4, 128),
+                             ([2049 + 198 * i for i in range(32)], 24, 4, 64), ([65521] * 16, 16, 4, 128), ([1000] * 64, 8, 4, 256)]:
+        b, width = len(lens), max(lens)
+        n_pages = sum(-(-n // 16) for n in lens)
+        order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(1))
+        table, at = torch.zeros(b, width, dtype=torch.int32), 0
+        for i, n in enumerate(lens):
+            p = -(-n // 16)
+            table[i, :n] = (order[at:at + p, None] * 16 + torch.arange(16)).reshape(-1)[:n].int()
+            at += p
+        table, rows, seq = table.cuda(), torch.arange(b, dtype=torch.int32, device="cuda"), torch.tensor(lens, device="cuda")
+        q = torch.randn(b, hq, d, device="cuda", generator=g).bfloat16()
+        four, slots = pools(n_pages * 16, hkv, d), torch.arange(n_pages * 16, device="cuda")
+        kb, vb = (torch.randn(n_pages * 16, hkv, d, device="cuda", generator=g, dtype=torch.bfloat16) for _ in "kv")
+        ops.kv4_append_(kb, vb, *four, slots)
+        o_part, ml, cnt = work = ops.kv4_decode_workspace(b, hq, hkv, d, "cuda")
+        out = torch.empty_like(q)
+        splits = int(op.paged_decode_splits(b, hkv, width, 32))
+        a = t(lambda: ops.kv4_decode(q, *four, table, rows, seq, max_len=width, workspace=work, out=out))
+        c = t(lambda: op.paged_decode_(q, kb, vb, table, rows, seq, d ** -0.5, splits, o_part, ml, cnt, out))
+        numbers = 2 * sum(lens) * hkv * d / 1e6
+        print(f"  {b:3d} of {min(lens):5d}..{width:5d} {hq}q/{hkv}kv D{d}: {a * 1e3:7.1f} us {numbers * 0.625 / a:5.0f} | {c * 1e3:7.1f} us {2 * numbers / c:5.0f}")
+    print("rows in / out (us, GB/s of rows and cache)")
+    for n, heads, d in [(16, 4, 128), (8192, 8, 128), (131072, 8, 128)]:
+        four = pools(n, heads, d)
+        k, v = (torch.randn(n, heads, d, device="cuda", generator=g, dtype=torch.bfloat16) for _ in "kv")
+        loc = torch.randperm(n, device="cuda", generator=g)
+        a, c = t(lambda: ops.kv4_append_(k, v, *four, loc)), t(lambda: ops.kv4_gather(*four, loc))
+        mb = 2 * n * heads * d * 2.625 / 1e6
+        print(f"  {n:6d} x {heads} x {d}: {a * 1e3:7.1f} us {mb / a:5.0f} | {c * 1e3:7.1f} us {mb / c:5.0f}")
+    print("page copies (us, GB/s read and written)")
+    for n, layers, heads in [(1, 24, 4), (192, 32, 8)]:
+        four = pools(512 * 16, heads, 128, layers)
+        a = t(lambda: ops.copy_pages_(four, list(range(n)), list(range(256, 256 + n)), 16))
+        print(f"  {n:3d} pages, {layers} layers {heads} x 128: {a * 1e3:7.1f} us {4 * n * 16 * layers * heads * 80 / 1e6 / a:5.0f}")
+
+
 if __name__ == "__main__":
-    table = {"gemm": bench_gemm, "skinny": bench_skinny, "flash": bench_flash, "fp8": bench_fp8, "quant": bench_quant, "sample": bench_sample, "decode": bench_decode}
+    table = {"gemm": bench_gemm, "skinny": bench_skinny, "flash": bench_flash, "fp8": bench_fp8, "quant": bench_quant, "sample": bench_sample, "decode": bench_decode, "kv4": bench_kv4}
     which = [a for a in sys.argv[1:] if not a.startswith("--")] or list(table)
     for name in which:
         table[name]()
