@@ -203,6 +203,65 @@ def test_long_and_many_requests(page):
         _near(ops.kv4_decode(q, *pools, table, rows, n), _expected(pools, table, rows, n, q, dim ** -0.5))
 
 
+def test_more_requests_than_threads_a_short_max_len_and_many_heads():
+    from astrai_b200 import ops
+
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 90, (300,), generator=g).tolist()  # a thread finds the place of several requests
+    lens[150] = 1500
+    for lens, heads, kv_heads, dim in ((lens, 2, 1, 64), ([500, 3, 0, 129], 128, 64, 32), ([40, 2], 512, 512, 32)):
+        pools, table, rows, n, q, _ = _case(lens, heads, kv_heads, dim, seed=31)
+        want = _expected(pools, table, rows, n, q, dim ** -0.5)
+        for parts, max_len in ((2, 0), (3, 7), (32, 1), (32, 0)):  # lengths beyond max_len are served all the same
+            work = ops.kv4_decode_workspace(len(lens) + 3, heads, kv_heads, dim, "cuda", parts=parts)  # and the workspace may be larger
+            _near(ops.kv4_decode(q, *pools, table, rows, n, max_len=max_len, workspace=work), want)
+            assert not work[2].any()
+
+
+def test_no_rows_views_of_a_projection_and_a_request_named_twice():
+    from astrai_b200 import ops
+
+    pools, table, rows, n, _, _ = _case([50, 9, 33], 4, 2, 64, seed=33)
+    before = [t.clone() for t in pools]
+    none = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    ops.kv4_append_(none, none, *pools, torch.empty(0, dtype=torch.int32, device="cuda"))
+    got = ops.kv4_gather(*pools, torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert [t.shape for t in got] == [(0, 2, 64)] * 2
+    qkv = _rows(3, 8, 64, seed=34)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    out = ops.kv4_decode(q, *pools, table, rows, n, k, v)
+    pools2 = [t.clone() for t in before]
+    assert torch.equal(out, ops.kv4_decode(q.contiguous(), *pools2, table, rows, n, k.contiguous(), v.contiguous()))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, pools2))
+    twice = rows[[0, 0, 2]]
+    _near(ops.kv4_decode(q, *pools, table, twice, n[[0, 0, 2]]), _expected(pools, table, twice, n[[0, 0, 2]], q, 64 ** -0.5))
+
+
+def test_a_graph_serves_lengths_that_grow_and_two_streams_run_side_by_side():
+    from astrai_b200 import ops
+
+    pools, table, rows, n, q, new = _case([900, 300, 0, 777], 8, 2, 128, seed=35)
+    full = n.clone()
+    n.copy_((full > 0).long())
+    work, out, g = ops.kv4_decode_workspace(4, 8, 2, 128, "cuda"), torch.empty_like(q), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.kv4_decode(q, *pools, table, rows, n, *new, workspace=work, out=out)
+    for part in (0.0, 0.3, 1.0):
+        n.copy_(torch.maximum((full * part).long(), (full > 0).long()))
+        g.replay()
+        _near(out, _expected(pools, table, rows, n, q, 128 ** -0.5))
+    n.copy_(full)
+    lanes = [(torch.cuda.Stream(), ops.kv4_decode_workspace(4, 8, 2, 128, "cuda"), torch.empty_like(q)) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, w, o in lanes:
+            with torch.cuda.stream(stream):
+                ops.kv4_decode(q, *pools, table, rows, n, workspace=w, out=o)
+    torch.cuda.synchronize()
+    assert torch.equal(lanes[0][2], lanes[1][2])
+    _near(lanes[0][2], _expected(pools, table, rows, n, q, 128 ** -0.5))
+
+
 @pytest.mark.parametrize("dim", DIMS)
 def test_numbers_far_from_one(dim):
     """Queries, keys and values of sizes from 2^-60 to 2^60, one step a thousand times another's."""
