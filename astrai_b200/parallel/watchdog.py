@@ -62,7 +62,10 @@ class Heartbeat:
     def leave(self, reason: str = "left"):
         """Announce an orderly exit so that the peers stop waiting at once instead of after ``timeout_s``."""
         self._left = True
-        self.store.set(f"{self.prefix}/{self.rank}", f"-1 {time.time():.3f} {reason}")
+        try:
+            self.store.set(f"{self.prefix}/{self.rank}", f"-1 {time.time():.3f} {reason}")
+        except RuntimeError as exc:  # the rank that hosts the store left first: nobody is there to be told
+            logger.warning("heartbeat: the store is gone, rank %d leaves unannounced: %s", self.rank, exc)
 
     # -- the peers ---------------------------------------------------------------------------------------------------------
     def _read(self, peer: int):

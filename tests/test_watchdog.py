@@ -90,3 +90,11 @@ def test_survivors_write_an_emergency_checkpoint_without_collectives(tmp_path, m
         assert not os.path.exists(os.path.join(root, "optimizer.pt"))
     else:
         assert os.path.getsize(os.path.join(root, "optimizer.pt")) > 0
+
+
+def test_a_rank_leaves_in_order_when_the_rank_that_hosts_the_store_left_first():
+    class Gone:
+        def set(self, key, value):
+            raise dist.DistNetworkError("Broken pipe")
+
+    Heartbeat(2, 3, store=Gone()).leave("finished")
