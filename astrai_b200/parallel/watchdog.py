@@ -62,10 +62,28 @@ class Heartbeat:
     def leave(self, reason: str = "left"):
         """Announce an orderly exit so that the peers stop waiting at once instead of after ``timeout_s``."""
         self._left = True
+        with self._lock:
+            dead = sorted(self._dead)
         try:
+            if dead:  # why it leaves: a peer that sees this exit first learns of the ranks that were lost before it
+                self.store.set(f"{self.prefix}/{self.rank}/lost", " ".join(map(str, dead)))
             self.store.set(f"{self.prefix}/{self.rank}", f"-1 {time.time():.3f} {reason}")
         except RuntimeError as exc:  # the rank that hosts the store left first: nobody is there to be told
             logger.warning("heartbeat: the store is gone, rank %d leaves unannounced: %s", self.rank, exc)
+
+    def outlast_survivors(self):
+        """Rank 0 hosts the default store: after a rank was lost it waits, ``timeout_s`` at most, until the survivors have
+        left too, so that they find out from the store and not from its absence."""
+        with self._lock:
+            dead = set(self._dead)
+        if not dead or self.rank != 0:
+            return
+        end = time.time() + self.timeout_s
+        while time.time() < end:
+            beats = [self._read(r) for r in range(1, self.world_size) if r not in dead]
+            if all(b is None or b[0] < 0 for b in beats):
+                return
+            time.sleep(min(0.05, self.interval_s))
 
     # -- the peers ---------------------------------------------------------------------------------------------------------
     def _read(self, peer: int):
@@ -77,6 +95,25 @@ class Heartbeat:
             return None
         parts = raw.split(" ", 2)
         return int(parts[0]), float(parts[1]), (parts[2] if len(parts) > 2 else "")
+
+    def _lost_before(self, peer: int) -> List[int]:
+        """The ranks that ``peer`` had found dead when it left."""
+        key = f"{self.prefix}/{peer}/lost"
+        try:
+            if hasattr(self.store, "check") and self.store.check([key]):
+                return [int(r) for r in self.store.get(key).decode().split()]
+        except Exception:  # noqa: BLE001 - as in _read
+            pass
+        return []
+
+    def _report(self, peer: int, why: str):
+        with self._lock:
+            if peer in self._dead:
+                return  # the other scanner (the thread, or a caller of scan) reported it a moment ago
+            self._dead[peer] = why
+        logger.error("heartbeat: rank %d %s", peer, why)
+        if self.on_failure is not None:
+            self.on_failure([peer])
 
     def scan(self) -> Dict[int, str]:
         """One pass over the peers; returns {rank: reason} of the ones considered dead so far."""
@@ -90,17 +127,14 @@ class Heartbeat:
             step, stamp, reason = got
             if step < 0:
                 why = f"announced its exit ({reason})"
+                for lost in self._lost_before(peer):
+                    if lost != self.rank:
+                        self._report(lost, f"was lost before rank {peer} left")
             elif now - stamp > self.timeout_s:
                 why = f"has not beaten for {now - stamp:.1f} s (last step {step})"
             else:
                 continue
-            with self._lock:
-                if peer in self._dead:
-                    continue  # the other scanner (the thread, or a caller of scan) reported it a moment ago
-                self._dead[peer] = why
-            logger.error("heartbeat: rank %d %s", peer, why)
-            if self.on_failure is not None:
-                self.on_failure([peer])
+            self._report(peer, why)
         with self._lock:
             return dict(self._dead)
 
@@ -200,6 +234,7 @@ class HeartbeatCallback:
     def on_train_end(self, context):
         if self.hb is not None:
             self.hb.leave("finished")
+            self.hb.outlast_survivors()
             self.hb.stop()
 
     def on_epoch_begin(self, context): ...

@@ -98,3 +98,19 @@ def test_a_rank_leaves_in_order_when_the_rank_that_hosts_the_store_left_first():
             raise dist.DistNetworkError("Broken pipe")
 
     Heartbeat(2, 3, store=Gone()).leave("finished")
+
+
+def test_a_rank_that_leaves_over_a_lost_rank_names_it():
+    """Rank 0 finds rank 1 silent and leaves; rank 2, whose own scan sees rank 0's exit first, learns of both."""
+    store = dist.HashStore()
+    a, b, c = (Heartbeat(r, 3, store=store, timeout_s=t) for r, t in ((0, 0.05), (1, 60.0), (2, 60.0)))
+    for h in (a, b, c):
+        h.beat(1)
+    time.sleep(0.1)
+    c.beat(2)
+    assert list(a.scan()) == [1]
+    a.leave("a rank was lost")
+    assert sorted(c.scan()) == [0, 1]
+    with pytest.raises(RankFailure) as exc:
+        c.check()
+    assert exc.value.ranks == [0, 1] and "was lost before rank 0 left" in str(exc.value)
