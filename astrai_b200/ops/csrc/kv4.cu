@@ -155,7 +155,7 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
 // accumulator's rounding.  lo_kg sum(q_hg) is a product of the (m, s) words as they lie in memory with (sum q, -8 sum q)
 // split into three bf16 parts (24 bits).
 //
-// Work: a request is its turns of UNIT = 32 W keys, counted in halves, and an empty one (what it costs to begin and end one);
+// Work: a request is ceil(len / UNIT) turns of UNIT = 32 W keys and SETUP empty ones (what it costs to begin and end one);
 // the requests of the batch, laid end to end, are divided evenly over groups of CTAs, whatever the lengths.  A group has a
 // CTA for each kv head: the rows of a token's heads lie side by side in memory and are read at about the same time (with
 // the heads' parts cut independently a batch of 16 x 65521 tokens took 211 us).  A CTA walks its range request by request:
@@ -170,7 +170,7 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
 // of 32 keys has a chain of products, a maximum over lanes, exponentials and products again).  Four warps a scheduler at
 // 128 registers spilled and took 190 us.  A launch begins with some 5 us of lengths, table, slots and first tiles and ends
 // with 3 to 4 us in which sums meet, and shorter work is bound by those: one request of 65521 tokens over 8 kv heads
-// 33.6 us (floor 12.8), 128 requests of 16 to 4608 tokens over 4 28.8 us (floor 11.8), 32 of 2049 to 8191 over 4 of 64
+// 34.7 us (floor 12.8), 128 requests of 16 to 4608 tokens over 4 28.8 us (floor 11.8), 32 of 2049 to 8191 over 4 of 64
 // numbers 26.8 us (floor 7.0), 64 of 1000 over 4 of 256 numbers 34.5 us, one of 8192 over 4 12.4 us, 4 of 1 to 33 6.2 us.
 //
 // Keys are the rows of the logits' product and queries its columns: a lane then holds two keys' steps, and eight query heads
@@ -349,9 +349,6 @@ template <int D, int W> __device__ __forceinline__ void kv4_join(const Kv4Attn& 
 // to 4608 took 28.8 us with 1 turn, 30.9 with 2, 34.5 with 3; 128 requests of 100 tokens 13.2, 11.5 and 13.0; cuts that are
 // not moved: 30.8 and 13.0).
 constexpr int KV4_SETUP = 1, KV4_TOL = 1;
-// A cut may fall between the halves of a turn (one request of 65521 tokens over 8 kv heads 34.7 -> 33.6 us; between its
-// quarters 33.9, but 128 mixed lengths 28.8 -> 30.7).
-constexpr int KV4_CUT = 2;
 // W warps a CTA; `per_sm` CTAs fit an SM: 128, 168 and 255 registers a thread for D up to 64, 128 and 256 (D = 64, 16
 // requests of 65521 tokens: three CTAs 116 us, four 105; shared memory that does not begin on a 128-byte line: 137).
 template <int D, int W> constexpr int kv4_per_sm() { return W == 12 ? 1 : D == 256 ? 2 : D == 128 ? 3 : 4; }
@@ -359,8 +356,8 @@ template <int D, int W> constexpr int kv4_per_sm() { return W == 12 ? 1 : D == 2
 template <int D, int W>
 __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(const Kv4Attn p) {
   using T = Kv4Tile<D>;
-  constexpr int NG = T::NG, NB = NG < 4 ? NG : 4, BATCHES = NG / NB, STAGES = T::STAGES, UNIT = 32 * W, STEP = UNIT / KV4_CUT;
-  constexpr int SETUP = KV4_SETUP * KV4_CUT, TOL = KV4_TOL * KV4_CUT;
+  constexpr int NG = T::NG, NB = NG < 4 ? NG : 4, BATCHES = NG / NB, STAGES = T::STAGES, UNIT = 32 * W;
+  constexpr int SETUP = KV4_SETUP, TOL = KV4_TOL;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t s_mask[W][STAGES];
   __shared__ float s_ml[W][8][2];
@@ -381,13 +378,13 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
     const long long n = p.lens[b];
     return row < 0 || row >= p.table_rows || n < 0 ? 0 : n > p.max_ctx ? p.max_ctx : (int)n;
   };
-  auto turns = [&](int len) -> int { return (len + STEP - 1) / STEP + SETUP; };
+  auto turns = [&](int len) -> int { return (len + UNIT - 1) / UNIT + SETUP; };
 
-  // Group i has the half turns from cut i to cut i + 1, where cut i lies at half turn i base + min(i, extra), moved to the end
-  // of its request if that is `tol` of them away or less: a cut costs a join.
+  // Group i has the turns from cut i to cut i + 1, where cut i lies at turn i base + min(i, extra), moved to the end of its
+  // request if that is `tol` turns away or less: a cut costs a join.
   const int group = blockIdx.x / p.heads, kvh = blockIdx.x - group * p.heads;
-  int u, u_end, b, start, base, extra;  // start: where the current request b begins
-  auto tol_of = [&](int n) -> int { return min(min(TOL, base >> 1), (n - 1) >> 1); };  // n: half turns of the request
+  int u, u_end, b, start, base, extra;  // start: first turn of the current request b
+  auto tol_of = [&](int n) -> int { return min(min(TOL, base >> 1), (n - 1) >> 1); };  // n: turns of the request
   {
     const int per = (p.batch + W * 32 - 1) / (W * 32);
     const int b0 = threadIdx.x * per;
@@ -417,7 +414,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
       const int i = group + k;
       cut[k] = i * base + min(i, extra);
       const int x = min(cut[k], total - 1);
-      if (x >= before && x < before + mine) {  // the request that the cut lies in, and where it begins
+      if (x >= before && x < before + mine) {  // the request that the cut lies in, and the request's first turn
         int at = before, r = b0;
         if (per > 1) {
           for (;; ++r) {
@@ -449,8 +446,8 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
     r.b = request, r.start = first;
     r.len = same(length(request)), r.row = same(p.rows[request]);
     r.behind = first + turns(r.len);
-    r.key_end = u_end >= r.behind ? r.len : max(0, u_end - first - SETUP) * STEP;
-    r.key = max(0, u - first - SETUP) * STEP + warp * 32;
+    r.key_end = u_end >= r.behind ? r.len : max(0, u_end - first - SETUP) * UNIT;
+    r.key = max(0, u - first - SETUP) * UNIT + warp * 32;
   };
 
   // ---- copies: a tile's slots, then its rows.  A key whose slot is outside the pool takes the row of one that is not
@@ -828,7 +825,7 @@ template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long r
     if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W / KV4_CUT) + 2 + KV4_SETUP * KV4_CUT) > 0x3fffffffLL) return -4;
+  if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
   const long long most = p.batch * ((max_len - 1) / (32 * W) + 1);  // units, if no request is longer
   long long groups = 148 * kv4_per_sm<D, W>() / p.heads;
   if (groups > room) groups = room;
@@ -840,7 +837,7 @@ template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long r
 }
 
 // Where the workspace has fewer parts than a wave of CTAs would make (few long requests), each is made by more warps: one
-// request of 65521 tokens over 8 kv heads, 32 parts, takes 34.7 us with 12 warps a CTA and 37.3 with 4 (cuts at whole turns).  Elsewhere a cut
+// request of 65521 tokens over 8 kv heads, 32 parts, takes 34.7 us with 12 warps a CTA and 37.3 with 4.  Elsewhere a cut
 // every 128 keys divides the work better than one every 384: 128 mixed requests 28.8 us with 4 warps, 39.1 with 12.
 template <int D> static int kv4_attn_pick(const Kv4Attn& p, int parts, long long max_len, cudaStream_t st) {
   const long long room = (long long)p.batch * (parts - 1) + 1;
