@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch import Tensor
 from torch.autograd import Function
 
@@ -75,11 +76,24 @@ def flash_attention_varlen(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
     d = q.shape[-1]
     scale = float(scale) if scale is not None else d ** -0.5
     batch = cu_seqlens_q.numel() - 1
-    cu_q, cu_k = cu_seqlens_q.int(), cu_seqlens_k.int()
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        # nothing to keep for a backward pass: serving's short prompts spend more time in Python than on the GPU
-        return torch.ops.astrai_b200.flash_fwd(_fix(q), _fix(k), _fix(v), cu_q, cu_k, batch, 0, 0, int(max_q), bool(causal), scale)[0]
-    return _FlashFn.apply(q, k, v, cu_q, cu_k, batch, 0, 0, int(max_q), int(max_k), bool(causal), scale)
+    return _FlashFn.apply(q, k, v, cu_seqlens_q.int(), cu_seqlens_k.int(), batch, 0, 0, int(max_q), int(max_k),
+                          bool(causal), scale)
+
+
+def derivatives_asked(*tensors: Tensor) -> bool:
+    """Whether reverse or forward mode follows what is computed from these."""
+    return any((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def flash_attention_ragged(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, max_q: int, max_k: int,
+                           scale: float) -> Tensor:
+    """Causal :func:`flash_attention_varlen` of a serving step: straight to the kernel where no derivative is asked for
+    (short prompts spend more time in Python than on the GPU), with it otherwise."""
+    if derivatives_asked(q, k, v):
+        return flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_q, max_k, causal=True, scale=scale)
+    native.require()
+    return torch.ops.astrai_b200.flash_fwd(_fix(q), _fix(k), _fix(v), cu_seqlens_q.int(), cu_seqlens_k.int(), cu_seqlens_q.numel() - 1,
+                                           0, 0, int(max_q), True, float(scale))[0]
 
 
 PAGED_PAGE_SIZES = (8, 16, 32, 64)

@@ -125,8 +125,7 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
             # the prompt's own rows are read back with the cached ones: a token sees the same numbers of a key whether its
             # prompt ran in one chunk or several
             kk, vv = kv4.kv4_gather(*pools, kv_cache.kv_gather_loc)
-            return flash.flash_attention_varlen(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens),
-                                                causal=True, scale=scale)
+            return flash.flash_attention_ragged(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens), scale)
     elif (native_on and attn_mask is None and fwd == "prefill" and kv_cache.qo_indptr is not None and page in flash.PAGED_PAGE_SIZES
             and flash.supported(q, kv_cache.k_buffer[layer_id], kv_cache.v_buffer[layer_id])):
         # ragged prefill over the paged pool: the kernel walks the slot table itself (no gathered copy of the keys)
@@ -139,8 +138,7 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
         # included) into packed tensors once, then one varlen launch with lower-right aligned causal masking
         kk = kv_cache.k_buffer[layer_id].index_select(0, kv_cache.kv_gather_loc)
         vv = kv_cache.v_buffer[layer_id].index_select(0, kv_cache.kv_gather_loc)
-        return flash.flash_attention_varlen(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens),
-                                            causal=True, scale=scale)
+        return flash.flash_attention_ragged(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens), scale)
     rows = kv_cache.req_pool_indices.tolist()
     outs, start = [], 0
     for i, (ql, kl) in enumerate(zip(q_lens, kv_lens)):
