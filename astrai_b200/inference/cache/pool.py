@@ -123,8 +123,12 @@ class PagePool:
                 ti += list(range(n))
             tile_b, tile_i = ws.put_int(ws.q_tile_to_batch, tb), ws.put_int(ws.q_tile_to_index, ti)
             gather = None
-            # the prefill kernel walks the table itself; rows of a 4-bit pool are read back into packed tensors first
-            in_place = not self.contiguous and self.page_size in (8, 16, 32, 64) and self.kv_dtype != "int4"
+            # the prefill kernel walks the table itself; rows of a 4-bit pool are read back into packed tensors first, unless
+            # there is one position of each request: those attend on the codes (up to 8 query heads a kv head)
+            if self.kv_dtype == "int4":
+                in_place = max(q_lens) == 1 and ws.max_q_heads // self.n_kv_heads <= 8
+            else:
+                in_place = not self.contiguous and self.page_size in (8, 16, 32, 64)
             if self.device.type == "cuda" and not in_place:  # one index for "all keys of the batch": gathered once per layer
                 gather = torch.cat([host[r, :n] for r, n in zip(req_indices, seq_lens)]).to(torch.int64).to(self.device, non_blocking=True)
             return KVCache(self._storage.k_buffer, self._storage.v_buffer, self._req_pool.req_to_token, rows, lens_t,

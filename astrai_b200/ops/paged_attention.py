@@ -8,15 +8,16 @@ Packed layout: ``q [T, Hq, D]``, ``k / v [T, Hkv, D]`` where the batch is concat
   kernel reads K / V straight from the pool through the slot table; other page sizes (and the contiguous layout's
   page size 1) gather the batch's keys into packed tensors first.  Head dims other than 64 / 128 and explicit masks
   take a per-request SDPA loop.
-* a 4-bit cache (:mod:`astrai_b200.ops.kv4`): decode attends on the codes, prefill stores the new rows, reads the batch's rows
-  back as bf16 and runs the same varlen launch.
+* a 4-bit cache (:mod:`astrai_b200.ops.kv4`): decode attends on the codes, and so does a prefill that has one position of
+  each request (forks, prompts found whole in the prefix index); any other prefill stores the new rows, reads the batch's
+  rows back as bf16, those of a bounded number of keys at a time, and runs the same varlen launch.
 The CPU statement of both is the same gather + softmax and is what the tests compare against
 (semantics of ``TorchNativeBackend`` in the reference, ``astrai/extension/backend/attention.py:443-498``).
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -85,6 +86,52 @@ def _decode_native_ok(q: Tensor, cache: KVCache) -> bool:
     )
 
 
+# Bytes of bf16 rows that a prefill over a 4-bit pool reads back at a time (a longer request's rows are read at once).  A
+# piece of few requests leaves the attention kernel few items: 16 requests of 64 positions behind 16320 (1 GB of rows, 32 / 8
+# heads of 128) take 0.80 ms in one piece, 0.83 in two, 1.07 in three and 1.73 in six; 8 of 128 behind 65408 (2 GB) 1.58 ms in one, 2.31 in
+# two, 4.13 in four.  Without a bound a batch behind long histories takes as much memory as a bf16 pool would.
+READ_BACK_BYTES = 1 << 30
+
+
+def read_back_pieces(kv_lens: Sequence[int], limit: int) -> List[Tuple[int, int]]:
+    """Ranges ``[first, last)`` of requests, about equal, that have at most ``limit`` keys together; a longer request has its own."""
+    total = sum(kv_lens)
+    share = total / max(1, -(-total // max(limit, 1)))
+    pieces, first, keys = [], 0, 0
+    for i, n in enumerate(kv_lens):
+        if i > first and (keys + n > limit or keys >= share):
+            pieces.append((first, i))
+            first, keys = i, 0
+        keys += n
+    return pieces + [(first, len(kv_lens))]
+
+
+def _read_back_attention(q: Tensor, pools, cache: KVCache, q_lens, kv_lens, scale: float) -> Tensor:
+    """Ragged prefill over a 4-bit pool.  The prompt's own rows are read back with the cached ones, so that a position sees
+    the same numbers of a key whether its prompt ran in one chunk or in several."""
+    heads, dim = pools[0].shape[1], q.shape[-1]
+    pieces = read_back_pieces(kv_lens, READ_BACK_BYTES // (4 * heads * dim))
+    if len(pieces) == 1:
+        return flash.flash_attention_ragged(q, *kv4.kv4_gather(*pools, cache.kv_gather_loc), cache.qo_indptr, cache.kv_indptr,
+                                            max(q_lens), max(kv_lens), scale)
+    outs, q0, k0 = [], 0, 0
+    for a, b in pieces:
+        q1, k1 = q0 + sum(q_lens[a:b]), k0 + sum(kv_lens[a:b])
+        outs.append(flash.flash_attention_ragged(q[q0:q1], *kv4.kv4_gather(*pools, cache.kv_gather_loc[k0:k1]), cache.qo_indptr[a:b + 1] - q0,
+                                                 cache.kv_indptr[a:b + 1] - k0, max(q_lens[a:b]), max(kv_lens[a:b]), scale))
+        q0, k0 = q1, k1
+    return torch.cat(outs)
+
+
+def _one_position_each(q: Tensor, cache: KVCache, q_lens) -> bool:
+    """A prefill that the decode kernel answers: one query of each request, no derivative asked for.  Heads of 128, 8 forks of
+    4096 positions (16 / 4 heads): 40 us, and 90 us with the rows read back; 64 of 16384 (32 / 8): 0.32 and 4.9 ms."""
+    hkv = cache.k_buffer.shape[2]
+    return (max(q_lens) == 1 and len(q_lens) == q.shape[0] and q.shape[1] % hkv == 0 and 1 <= q.shape[1] // hkv <= 8
+            and cache.seq_lens.dtype == torch.int64 and cache.req_pool_indices.dtype == torch.int32
+            and not flash.derivatives_asked(q))
+
+
 def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_id: int = 0,
                      attn_mask: Optional[Tensor] = None, is_causal: bool = True, fwd: str = "prefill") -> Tensor:
     if kv_cache is None:
@@ -120,12 +167,12 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
     q_lens, kv_lens = _lens(kv_cache)
     page = getattr(kv_cache, "page_size", 1) or 1
     if pools is not None:
-        if (native_on and attn_mask is None and fwd == "prefill" and kv_cache.kv_gather_loc is not None
-                and kv_cache.qo_indptr is not None and q.is_cuda and q.dtype == torch.bfloat16 and q.shape[-1] in flash.SUPPORTED_HEAD_DIMS):
-            # the prompt's own rows are read back with the cached ones: a token sees the same numbers of a key whether its
-            # prompt ran in one chunk or several
-            kk, vv = kv4.kv4_gather(*pools, kv_cache.kv_gather_loc)
-            return flash.flash_attention_ragged(q, kk, vv, kv_cache.qo_indptr, kv_cache.kv_indptr, max(q_lens), max(kv_lens), scale)
+        if native_on and attn_mask is None and fwd == "prefill" and q.is_cuda and q.dtype == torch.bfloat16:
+            if _one_position_each(q, kv_cache, q_lens):
+                return kv4.kv4_decode(q, *pools, kv_cache.req_to_token, kv_cache.req_pool_indices, kv_cache.seq_lens, scale=scale,
+                                      max_len=max(kv_lens))
+            if kv_cache.kv_gather_loc is not None and kv_cache.qo_indptr is not None and q.shape[-1] in flash.SUPPORTED_HEAD_DIMS:
+                return _read_back_attention(q, pools, kv_cache, q_lens, kv_lens, scale)
     elif (native_on and attn_mask is None and fwd == "prefill" and kv_cache.qo_indptr is not None and page in flash.PAGED_PAGE_SIZES
             and flash.supported(q, kv_cache.k_buffer[layer_id], kv_cache.v_buffer[layer_id])):
         # ragged prefill over the paged pool: the kernel walks the slot table itself (no gathered copy of the keys)

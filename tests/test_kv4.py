@@ -392,3 +392,12 @@ def test_commands_hand_the_options_on(tmp_path, monkeypatch):
     assert got["kv_dtype"] == "int4"
     assert CliRunner().invoke(serve.serve_command, ["--param_path", str(tmp_path), "--kv_dtype", "int3"]).exit_code == 2
     assert all(any(p.name == "kv_dtype" for p in bench.commands[c].params) for c in ("prefill", "decode", "serve"))
+
+
+def test_histories_are_read_back_in_pieces_of_a_bounded_number_of_keys():
+    from astrai_b200.ops.paged_attention import read_back_pieces
+
+    assert read_back_pieces([3, 4, 3], 10) == [(0, 3)] and read_back_pieces([3, 4, 4], 10) == [(0, 2), (2, 3)]
+    assert read_back_pieces([30, 4, 4, 11, 1], 10) == [(0, 1), (1, 3), (3, 4), (4, 5)]  # a longer request has its own
+    assert read_back_pieces([4, 4, 4, 4], 12) == [(0, 2), (2, 4)]  # and the pieces are about equal
+    assert read_back_pieces([7], 0) == [(0, 1)] and read_back_pieces([1, 1], 0) == [(0, 1), (1, 2)]
