@@ -20,7 +20,7 @@ from __future__ import annotations
 import logging
 import threading
 import time
-from typing import Callable, Dict, List, Optional
+from typing import Callable, Dict, List, Optional, Set, Tuple
 
 import torch.distributed as dist
 
@@ -43,6 +43,8 @@ class Heartbeat:
         self.rank, self.world_size, self.store = rank, world_size, store
         self.timeout_s, self.interval_s, self.on_failure, self.prefix = float(timeout_s), float(interval_s), on_failure, prefix
         self._dead: Dict[int, str] = {}
+        self._silent: Dict[int, str] = {}  # those of them that stopped beating: the time of their last beat, as they wrote it
+        self._finished: Set[int] = set()   # those of them that left because their work was done
         self._stop = threading.Event()
         self._thread: Optional[threading.Thread] = None
         self._lock = threading.Lock()
@@ -60,28 +62,32 @@ class Heartbeat:
             self.store.set(f"{self.prefix}/{self.rank}", f"{self.step} {time.time():.3f}")
 
     def leave(self, reason: str = "left"):
-        """Announce an orderly exit so that the peers stop waiting at once instead of after ``timeout_s``."""
+        """Announce an orderly exit so that the peers stop waiting at once instead of after ``timeout_s``.  The first reason
+        that is given stands."""
+        if self._left:
+            return
         self._left = True
         with self._lock:
-            dead = sorted(self._dead)
+            silent = sorted(self._silent.items())
         try:
-            if dead:  # why it leaves: a peer that sees this exit first learns of the ranks that were lost before it
-                self.store.set(f"{self.prefix}/{self.rank}/lost", " ".join(map(str, dead)))
+            if silent:  # why it leaves: a peer that sees this exit first learns of the ranks that were lost before it
+                self.store.set(f"{self.prefix}/{self.rank}/lost", " ".join(f"{r}@{stamp}" for r, stamp in silent))
             self.store.set(f"{self.prefix}/{self.rank}", f"-1 {time.time():.3f} {reason}")
         except RuntimeError as exc:  # the rank that hosts the store left first: nobody is there to be told
             logger.warning("heartbeat: the store is gone, rank %d leaves unannounced: %s", self.rank, exc)
 
     def outlast_survivors(self):
-        """Rank 0 hosts the default store: after a rank was lost it waits, ``timeout_s`` at most, until the survivors have
-        left too, so that they find out from the store and not from its absence."""
+        """Rank 0 hosts the default store: after a rank was lost (went silent, or left before its work was done) it waits,
+        ``timeout_s`` at most, until the others have left or are lost too, so that they find out from the store and not from
+        its absence."""
         with self._lock:
-            dead = set(self._dead)
-        if not dead or self.rank != 0:
+            lost = set(self._dead) - self._finished
+        if not lost or self.rank != 0:
             return
         end = time.time() + self.timeout_s
         while time.time() < end:
-            beats = [self._read(r) for r in range(1, self.world_size) if r not in dead]
-            if all(b is None or b[0] < 0 for b in beats):
+            gone = self.scan()
+            if all(r in gone or self._read(r) is None for r in range(1, self.world_size)):
                 return
             time.sleep(min(0.05, self.interval_s))
 
@@ -96,21 +102,33 @@ class Heartbeat:
         parts = raw.split(" ", 2)
         return int(parts[0]), float(parts[1]), (parts[2] if len(parts) > 2 else "")
 
-    def _lost_before(self, peer: int) -> List[int]:
-        """The ranks that ``peer`` had found dead when it left."""
+    def _lost_before(self, peer: int) -> List[Tuple[int, str]]:
+        """The ranks that ``peer`` had found silent when it left, each with the time of its last beat."""
         key = f"{self.prefix}/{peer}/lost"
         try:
             if hasattr(self.store, "check") and self.store.check([key]):
-                return [int(r) for r in self.store.get(key).decode().split()]
+                return [(int(r), stamp) for r, stamp in (item.split("@") for item in self.store.get(key).decode().split())]
         except Exception:  # noqa: BLE001 - as in _read
             pass
         return []
 
-    def _report(self, peer: int, why: str):
+    def _hear(self, lost: int, stamp: str, peer: int):
+        """``peer`` left and says that ``lost`` has not beaten since ``stamp``.  What the rank says itself comes first: an exit
+        that it announced is found by the scan, and a beat after ``stamp`` shows that it was only slow (both times are the
+        rank's own, so clocks are not compared)."""
+        got = self._read(lost)
+        if got is None or (got[0] >= 0 and f"{got[1]:.3f}" == stamp):
+            self._report(lost, f"was lost before rank {peer} left", silent=stamp)
+
+    def _report(self, peer: int, why: str, silent: Optional[str] = None, finished: bool = False):
         with self._lock:
             if peer in self._dead:
                 return  # the other scanner (the thread, or a caller of scan) reported it a moment ago
             self._dead[peer] = why
+            if silent is not None:
+                self._silent[peer] = silent
+            if finished:
+                self._finished.add(peer)
         logger.error("heartbeat: rank %d %s", peer, why)
         if self.on_failure is not None:
             self.on_failure([peer])
@@ -126,15 +144,12 @@ class Heartbeat:
                 continue  # has not started beating yet: start-up is covered by the rendezvous timeout
             step, stamp, reason = got
             if step < 0:
-                why = f"announced its exit ({reason})"
-                for lost in self._lost_before(peer):
+                for lost, last in self._lost_before(peer):
                     if lost != self.rank:
-                        self._report(lost, f"was lost before rank {peer} left")
+                        self._hear(lost, last, peer)
+                self._report(peer, f"announced its exit ({reason})", finished=reason == "finished")
             elif now - stamp > self.timeout_s:
-                why = f"has not beaten for {now - stamp:.1f} s (last step {step})"
-            else:
-                continue
-            self._report(peer, why)
+                self._report(peer, f"has not beaten for {now - stamp:.1f} s (last step {step})", silent=f"{stamp:.3f}")
         with self._lock:
             return dict(self._dead)
 

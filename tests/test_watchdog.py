@@ -114,3 +114,110 @@ def test_a_rank_that_leaves_over_a_lost_rank_names_it():
     with pytest.raises(RankFailure) as exc:
         c.check()
     assert exc.value.ranks == [0, 1] and "was lost before rank 0 left" in str(exc.value)
+
+
+def test_a_report_names_only_ranks_that_went_silent_and_yields_to_what_the_rank_says_itself():
+    """A rank that finished is not reported as lost, and a rank that beat after it was given up for lost is believed."""
+    store = dist.HashStore()
+    a, b, c, d = (Heartbeat(r, 4, store=store, timeout_s=t) for r, t in ((0, 0.05), (1, 60.0), (2, 60.0), (3, 60.0)))
+    for h in (a, b, c, d):
+        h.beat(1)
+    b.leave("finished")
+    time.sleep(0.1)
+    c.beat(2)
+    assert sorted(a.scan()) == [1, 3]  # one has finished, one is silent
+    a.leave("a rank was lost")
+    time.sleep(0.01)
+    d.beat(2)  # it was only slow
+    got = c.scan()
+    assert sorted(got) == [0, 1] and got[1] == "announced its exit (finished)"
+    d.leave("finished")
+    assert c.scan()[3] == "announced its exit (finished)"
+
+
+def test_a_report_is_handed_on():
+    """Rank 0 finds rank 1 silent, rank 2 learns of it from rank 0, rank 3 from rank 2 alone."""
+    store = dist.HashStore()
+    a, b, c, d = (Heartbeat(r, 4, store=store, timeout_s=t) for r, t in ((0, 0.05), (1, 60.0), (2, 60.0), (3, 60.0)))
+    for h in (a, b, c, d):
+        h.beat(1)
+    time.sleep(0.1)
+    c.beat(2), d.beat(2)
+    assert sorted(a.scan()) == [1]
+    a.leave("error")
+    assert sorted(c.scan()) == [0, 1]
+    store.delete_key("hb/0")
+    c.leave("error")
+    assert sorted(d.scan()) == [1, 2] and "was lost before rank 2 left" in d.scan()[1]
+
+
+def test_the_first_exit_that_a_rank_announces_stands():
+    store = dist.HashStore()
+    a, b = (Heartbeat(r, 2, store=store) for r in range(2))
+    a.beat(1), b.beat(1)
+    b.leave("error")
+    b.leave("finished")
+    assert a.scan()[1] == "announced its exit (error)"
+
+
+@pytest.mark.parametrize("lost", ["silent", "error"])
+def test_the_rank_that_hosts_the_store_waits_for_the_survivors(lost):
+    import threading
+
+    store = dist.HashStore()
+    a, b, c, d = (Heartbeat(r, 4, store=store, timeout_s=2.0) for r in range(4))
+    for h in (a, b, c, d):
+        h.beat(1)
+    if lost == "error":
+        b.leave("error")
+    else:
+        time.sleep(2.1)
+        for h in (a, c, d):
+            h.beat(2)
+    assert sorted(a.scan()) == [1]
+    a.leave("a rank was lost")
+    threading.Timer(0.15, c.leave, ["a rank was lost"]).start()
+    threading.Timer(0.3, d.leave, ["a rank was lost"]).start()
+    start = time.time()
+    a.outlast_survivors()
+    assert 0.25 < time.time() - start < 1.5  # until the last of them has left, not until the timeout
+    start = time.time()
+    c.outlast_survivors()  # a rank that hosts nothing does not wait
+    assert time.time() - start < 1.0
+
+
+def test_the_wait_for_survivors_ends_with_one_that_is_lost_meanwhile_and_at_the_timeout():
+    store = dist.HashStore()
+    a, b, c = (Heartbeat(r, 3, store=store, timeout_s=3.0) for r in range(3))
+    for h in (a, b, c):
+        h.beat(1)
+    b.leave("error")
+    time.sleep(2.0)
+    assert sorted(a.scan()) == [1]
+    start = time.time()
+    a.outlast_survivors()  # rank 2 has been silent for 2 s: it is lost a second from now
+    assert 0.8 < time.time() - start < 2.5 and sorted(a.dead_ranks()) == [1, 2]
+    store = dist.HashStore()
+    a, b, c = (Heartbeat(r, 3, store=store, timeout_s=t) for r, t in ((0, 0.3), (1, 60.0), (2, 60.0)))
+    for h in (a, b, c):
+        h.beat(1)
+    b.leave("error")
+    a.scan()
+    c._publish = lambda: store.set("hb/2", f"1 {time.time() + 100:.3f}")  # alive, and never leaving
+    c._publish()
+    start = time.time()
+    a.outlast_survivors()
+    assert 0.25 < time.time() - start < 5.0
+
+
+def test_ranks_that_finish_in_order_are_not_waited_for():
+    store = dist.HashStore()
+    a, b, c = (Heartbeat(r, 3, store=store, timeout_s=60.0) for r in range(3))
+    for h in (a, b, c):
+        h.beat(1)
+    b.leave("finished")
+    assert sorted(a.scan()) == [1]
+    a.leave("finished")
+    start = time.time()
+    a.outlast_survivors()
+    assert time.time() - start < 5.0
