@@ -10,6 +10,7 @@ one token, which keeps CUDA-graph replay valid.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Dict, List, Optional
 
@@ -88,9 +89,22 @@ class PagePool:
     req_pool = property(lambda self: self._req_pool)
     storage = property(lambda self: self._storage)
 
-    def copy_pages(self, src: List[int], dst: List[int]):
-        """Copy pages in every layer (contiguous layout: whole rows), on the current stream."""
-        copy_pages_(self._storage.pools(), src, dst, self.max_seq_len if self.contiguous else self.page_size)
+    def copy_pages(self, src: List[int], dst: List[int], length: Optional[int] = None):
+        """Copy pages in every layer, on the current stream.  A page of the contiguous layout is a request's whole row, of
+        which the first ``length`` positions are copied (default: all)."""
+        size = self.page_size
+        if self.contiguous:
+            size = self._row_part(self.max_seq_len if length is None else length)
+            first, parts = self.max_seq_len // size, -(-(self.max_seq_len if length is None else length) // size)
+            src, dst = ([r * first + i for r in rows for i in range(parts)] for rows in (src, dst))
+        copy_pages_(self._storage.pools(), src, dst, size)
+
+    def _row_part(self, length: int) -> int:
+        """The parts in which the first ``length`` positions of a contiguous row are copied: they divide the row, hold 16
+        positions or more (fewer cost a thread block each for little) and number 256 at most (one launch)."""
+        n = self.max_seq_len
+        small = [d for d in range(1, math.isqrt(n) + 1) if n % d == 0]
+        return min(d for d in (*small, *(n // d for d in small)) if d == n or (d >= 16 and -(-length // d) <= 256))
 
     def bind_tasks(self, req_indices: List[int], seq_lens: List[int], workspace: InferenceWorkspace, device=None,
                    start_pos: Optional[int] = None, incremental: bool = False,

@@ -266,9 +266,9 @@ class AllocationStrategy:
     def extend(self, state: TaskCacheState, pos: int) -> bool:
         raise NotImplementedError
 
-    def fork(self, src: TaskCacheState, dst: TaskCacheState, length: int, copy: Callable[[List[int], List[int]], None]) -> bool:
-        """Give ``dst`` the first ``length`` positions of ``src``; ``copy(sources, destinations)`` copies what they cannot
-        share.  False when there is no room."""
+    def fork(self, src: TaskCacheState, dst: TaskCacheState, length: int, copy: Callable[..., None]) -> bool:
+        """Give ``dst`` the first ``length`` positions of ``src``; ``copy(sources, destinations)`` copies the pages that they
+        cannot share (``PagePool.copy_pages``).  False when there is no room."""
         raise NotImplementedError
 
     def write_indices(self, state: TaskCacheState, prompt_ids: List[int]) -> None:
@@ -292,7 +292,7 @@ class ContiguousStrategy(AllocationStrategy):
 
     def fork(self, src, dst, length, copy):
         if length:
-            copy([src.req_idx], [dst.req_idx])  # a row of the contiguous layout is one page
+            copy([src.req_idx], [dst.req_idx], length)  # a row of the contiguous layout is one page
         return True
 
     def write_indices(self, state, prompt_ids):

@@ -401,3 +401,23 @@ def test_histories_are_read_back_in_pieces_of_a_bounded_number_of_keys():
     assert read_back_pieces([30, 4, 4, 11, 1], 10) == [(0, 1), (1, 3), (3, 4), (4, 5)]  # a longer request has its own
     assert read_back_pieces([4, 4, 4, 4], 12) == [(0, 2), (2, 4)]  # and the pieces are about equal
     assert read_back_pieces([7], 0) == [(0, 1)] and read_back_pieces([1, 1], 0) == [(0, 1), (1, 2)]
+
+
+@pytest.mark.parametrize("kv_dtype", ["auto", "int4"])
+@pytest.mark.parametrize("row,length,copied", [(64, 20, 32), (64, 0, 0), (64, 64, 64), (7, 3, 7), (31, 5, 31), (8192, 5000, 5024), (8192, 100, 112)])
+def test_a_contiguous_fork_copies_no_more_than_its_length_asks_for(row, length, copied, kv_dtype):
+    """Rows are copied in equal parts (16 positions or more, 256 parts at most), not whole."""
+    from astrai_b200.inference.cache import PagePool, TaskCacheManager
+
+    pool = PagePool(2, 1, 32, 3, row, "cpu", torch.float32, kv_dtype=kv_dtype)
+    tc = TaskCacheManager(pool)
+    assert tc.task_alloc("a", list(range(length)))
+    for t in pool.storage.pools():
+        t.copy_(torch.randint(1, 100, t.shape))
+    before = [t.clone() for t in pool.storage.pools()]
+    assert tc.task_fork("a", "b")
+    a, b = tc.state("a").req_idx * row, tc.state("b").req_idx * row
+    for t, old in zip(pool.storage.pools(), before):
+        assert torch.equal(t[:, b:b + copied], old[:, a:a + copied])
+        t[:, b:b + copied] = old[:, b:b + copied]
+        assert torch.equal(t, old)  # nothing else has changed
