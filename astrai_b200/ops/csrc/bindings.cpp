@@ -460,7 +460,7 @@ void kv4_decode_(const Tensor& q_, Tensor& k_codes, Tensor& k_meta, Tensor& v_co
               "kv4_decode: out must be a contiguous bf16 tensor of q's shape");
   TORCH_CHECK(k_new.has_value() == v_new.has_value(), "kv4_decode: k_new and v_new come together");
   if (k_new) kv4_check_new("kv4_decode", *k_new, *v_new, k_codes, B, p);
-  TORCH_CHECK(B <= 65535 && req_to_token.size(0) <= INT32_MAX && req_to_token.size(1) <= INT32_MAX, "kv4_decode: batch or table too large");
+  TORCH_CHECK(B <= 65535 && req_to_token.size(0) <= INT32_MAX && req_to_token.size(1) <= ab::kKv4Positions, "kv4_decode: batch or table too large");
   TORCH_CHECK(B == 0 || (req_to_token.size(0) > 0 && req_to_token.size(1) > 0), "kv4_decode: req_to_token is empty");
   const c10::cuda::CUDAGuard guard(dev);
   const int given = o_part_.has_value() + ml_part_.has_value() + counters_.has_value();

@@ -814,6 +814,7 @@ __global__ void __launch_bounds__(W * 32, kv4_per_sm<D, W>()) kv4_attn_kernel(co
   }
 }
 
+static_assert(kKv4Positions <= 0x7fffffffLL - 4 * 32 * 12, "no position that a warp asks for passes 32 bits");
 template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long room, long long max_len, cudaStream_t st) {
   constexpr int bytes = W * Kv4Tile<D>::WARP + Kv4Tile<D>::QUERY;
   static_assert(Kv4Tile<D>::SPACE >= 4 * D * 4 && Kv4Tile<D>::SPACE >= 32 * 32, "a warp's space holds four heads of its sums");
@@ -825,7 +826,8 @@ template <int D, int W> static int kv4_attn_launch(const Kv4Attn& p, long long r
     if (cudaFuncSetAttribute(kv4_attn_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -5;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  if (p.max_ctx > 0x7fffff00 || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
+  // positions are counted in 32 bits, up to three turns behind a request's last one
+  if (p.max_ctx > kKv4Positions || p.batch * (p.max_ctx / (32LL * W) + 4) > 0x3fffffffLL) return -4;
   const long long most = p.batch * ((max_len - 1) / (32 * W) + 1);  // units, if no request is longer
   long long groups = 148 * kv4_per_sm<D, W>() / p.heads;
   if (groups > room) groups = room;

@@ -283,6 +283,7 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
 // aligned, used as flat arrays; counters int32 [batch * n_kv_heads], zero before the first call.  max_len sizes the grid
 // (0: the table's width); longer requests are served all the same.  k_new / v_new (both or neither): bf16 [batch, n_kv_heads, D],
 // stored into the slot of the last position first.  Returns also -1: more than 8 query heads per kv head, -2: parts.
+constexpr long long kKv4Positions = 0x7ffff000;  // the widest table
 int kv4_decode(const void* q, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const int* req_to_token, const int* req_pool_indices,
                const long long* seq_lens, const void* k_new, const void* v_new, float* o_part, float* ml_part, int* counters, void* out,
                int batch, int n_q_heads, int n_kv_heads, int head_dim, int max_ctx, int table_rows, long long n_slots, float scale, int parts,

@@ -100,3 +100,14 @@ def test_a_batch_reads_its_histories_back_in_bounded_pieces(monkeypatch):
     for i in range(len(lens)):
         o, tol = _expected(pool, kv, q, counts, lens, i, dim ** -0.5)
         assert ((out[sum(counts[:i]):sum(counts[:i + 1])].double() - o).abs() <= tol).all()
+
+
+def test_a_table_whose_positions_would_pass_32_bits_is_refused():
+    """Positions are counted in 32 bits, some turns beyond a request's last one; the table itself is never read here."""
+    from astrai_b200 import ops
+
+    pools = [t for _ in "kv" for t in (torch.zeros(16, 1, 32, dtype=torch.uint8, device="cuda"), torch.zeros(16, 1, 2, 2, dtype=torch.bfloat16, device="cuda"))]
+    q, rows = _rows(1, 1, 64, seed=1), torch.zeros(1, dtype=torch.int32, device="cuda")
+    table = torch.empty(1, 2 ** 31 - 512, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="table too large"):
+        ops.kv4_decode(q, *pools, table, rows, torch.zeros(1, dtype=torch.int64, device="cuda"))
