@@ -110,6 +110,8 @@ def kv4_gather(k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_meta: Tensor,
     outside the pool reads as zeros."""
     if k_codes.is_cuda:
         return _op("kv4_gather")(k_codes, k_meta, v_codes, v_meta, loc)
+    if loc.dim() != 1:
+        raise ValueError("kv4_gather: loc must be [tokens]")
     ok = _inside(loc, k_codes.shape[0])
     at = torch.where(ok, loc, torch.zeros_like(loc)).long()
     k, v = dequantize(k_codes[at], k_meta[at], True), dequantize(v_codes[at], v_meta[at], False)
@@ -148,12 +150,16 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
         _op("kv4_decode_")(q, k_codes, k_meta, v_codes, v_meta, req_to_token, req_pool_indices, seq_lens, k_new, v_new, scale,
                            max_len, o_part, ml_part, counters, out)
         return out
-    b, hq, d = q.shape
     hkv, slots = k_codes.shape[1], k_codes.shape[0]
+    if q.dim() != 3 or req_to_token.dim() != 2 or not req_pool_indices.shape == seq_lens.shape == q.shape[:1]:
+        raise ValueError("kv4_decode: q must be [batch, heads, head_dim], req_to_token [rows, positions], req_pool_indices and seq_lens [batch]")
+    b, hq, d = q.shape
     if d != 2 * k_codes.shape[2] or hq % hkv:
         raise ValueError("kv4_decode: q must be [batch, heads, head_dim] with heads a multiple of the pools' heads")
     if (k_new is None) != (v_new is None):
         raise ValueError("kv4_decode: k_new and v_new come together")
+    if any(t is not None and t.shape != (b, hkv, d) for t in (k_new, v_new)) or (out is not None and out.shape != q.shape):
+        raise ValueError("kv4_decode: k_new / v_new must be [batch, kv_heads, head_dim] and out of q's shape")
     width, rows = req_to_token.shape[1], req_to_token.shape[0]
     res = torch.zeros_like(q, memory_format=torch.contiguous_format) if out is None else out.zero_()
     spans = []

@@ -421,3 +421,20 @@ def test_a_contiguous_fork_copies_no_more_than_its_length_asks_for(row, length, 
         assert torch.equal(t[:, b:b + copied], old[:, a:a + copied])
         t[:, b:b + copied] = old[:, b:b + copied]
         assert torch.equal(t, old)  # nothing else has changed
+
+
+def test_shapes_that_do_not_fit_are_refused_on_the_cpu_too():
+    from astrai_b200 import ops
+
+    pools = _pools(16, 2, 32)
+    q, table, rows, lens = torch.randn(3, 4, 32), torch.arange(12).int().view(3, 4), torch.arange(3).int(), torch.tensor([4, 2, 1])
+    new = torch.randn(3, 2, 32).bfloat16()
+    before = [t.clone() for t in pools]
+    for bad in (dict(seq_lens=lens[:2]), dict(req_pool_indices=rows[:2]), dict(q=q[:2]), dict(q=q[0]), dict(req_to_token=table[0]),
+                dict(k_new=new[:2], v_new=new[:2]), dict(out=torch.empty(2, 4, 32)), dict(seq_lens=lens[:, None])):
+        with pytest.raises(ValueError, match="kv4_decode"):
+            ops.kv4_decode(**{**dict(q=q, k_codes=pools[0], k_meta=pools[1], v_codes=pools[2], v_meta=pools[3], req_to_token=table,
+                                     req_pool_indices=rows, seq_lens=lens), **bad})
+    with pytest.raises(ValueError, match="kv4_gather"):
+        ops.kv4_gather(*pools, rows[:, None])
+    assert all(torch.equal(t, b) for t, b in zip(pools, before))
