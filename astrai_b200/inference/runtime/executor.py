@@ -189,7 +189,8 @@ class Executor:
         ws = self._workspace
         return dataclasses.replace(kv, req_pool_indices=ws.req_pool_indices[:rows], seq_lens=ws.seq_lens[:rows],
                                    out_cache_loc=ws.out_cache_loc[:rows], qo_indptr=ws.qo_indptr[: rows + 1],
-                                   decode_splits=self._decode_splits(rows), max_len=0)  # a graph outlives the lengths of its capture
+                                   decode_splits=self._decode_splits(rows),
+                                   max_len=self.kv_cache.max_seq_len)  # a graph outlives the lengths of its capture
 
     def _zero_padding(self, b: int, rows: int):
         ws = self._workspace

@@ -438,3 +438,12 @@ def test_shapes_that_do_not_fit_are_refused_on_the_cpu_too():
     with pytest.raises(ValueError, match="kv4_gather"):
         ops.kv4_gather(*pools, rows[:, None])
     assert all(torch.equal(t, b) for t, b in zip(pools, before))
+
+
+def test_a_captured_step_is_told_the_longest_length_a_request_can_have(model):
+    """A graph outlives the lengths of its capture: a back end that sizes its work by ``max_len`` gets a bound that holds."""
+    sched = _scheduler(model)
+    ex = sched._executor
+    assert ex.task_cache.task_alloc("a", [1, 2, 3])
+    kv = ex.task_cache.bind(["a"], ex.workspace)
+    assert kv.max_len == 3 and ex._padded(kv, 1, 2).max_len == 48
