@@ -148,9 +148,13 @@ int kv4_gather(const void* k_codes, const void* k_meta, const void* v_codes, con
 //   logit = sum_g s_kg (q_hg . c_kg) + lo_kg sum(q_hg)       out_d = sum_k (p_k s_kg) c_kd + sum_k p_k lo_kg   (d in g)
 // so the big products take the codes as they are: a code in the low bits of an fp16 IS the number c 2^-24 (a subnormal),
 // and one shifted left by four is c 2^-20, so a pair of numbers costs one AND (and every second pair a shift).  The
-// other operand is the query times a power of two that puts its largest number below 2^14 (exact), or p s times a power
-// of two that puts the tile's largest step below 2^15 (rounded to fp16: 2^-11 of each product; the query's and the
-// steps' own sizes cost nothing).  Products go to m16n8k16 tensor instructions with fp32 sums: a tile's share of `out` is
+// other operand is the query times a power of two that puts its largest number into [2^13, 2^14), or p s times a power of two
+// that puts the largest step of the tile's 32 rows into [2^14, 2^15), rounded to fp16.  What that costs (p: the weight
+// relative to the largest so far, 1):
+//   p s      2^-11 of it, and 2^-39 of the tile's largest step where it is below 2^-28 of that step
+//   query    nothing down to 2^-26 of the head's largest number, 2^-34 of that number below
+// so the sizes of queries, keys and values cost nothing by themselves, and ranges inside a head or a tile nothing that
+// bf16 numbers of one model come near.  Products go to m16n8k16 tensor instructions with fp32 sums: a tile's share of `out` is
 // summed from zero and added to the running sum in fp32 registers, so a long context loses nothing to the tensor
 // accumulator's rounding.  lo_kg sum(q_hg) is a product of the (m, s) words as they lie in memory with (sum q, -8 sum q)
 // split into three bf16 parts (24 bits).

@@ -136,7 +136,9 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
     ``req_to_token[req_pool_indices[i], :seq_lens[i]]`` (int32).  ``k_new`` / ``v_new [batch, kv_heads, D]`` are stored
     into the last position's slot first (when absent, the pool already holds them; two requests must not store into one slot).  A request of length 0 gives zeros;
     positions whose slot is outside the pool are left out.  The numbers of the cache enter unrounded, sums and softmax are
-    fp32, the result is bf16.
+    fp32, the result is bf16.  A value's weight times its group's step is rounded to fp16 (2^-11 of it; where it is below
+    2^-28 of the largest step among 32 neighbouring positions of the head, 2^-39 of that step), and query numbers below 2^-26
+    of their head's largest are rounded (2^-34 of that number).
 
     The keys of the whole batch are spread evenly over the GPU, whatever the lengths.  ``max_len``: the longest length, when
     the host knows it (0: the table's width) - it sizes the launch, a longer request is served all the same.  ``workspace``:

@@ -496,3 +496,41 @@ def test_serving_run_with_graphs_forks_and_chunks():
     forked = sched.run_batch(prompts[:2], max_tokens=12, temperature=0.0, samples_per_prompt=3)
     assert all(len(a) == 12 for a in forked)
     assert native.kernel_status("cuda") == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("gap", [0, 12, 20, 26, 30, 34, 40, 60])
+def test_ranges_inside_a_tile_and_a_head(gap, dim):
+    """Steps of one group 2^gap below another's, and query numbers 2^gap below the head's largest with keys as far above.
+
+    ``p s`` is rounded to fp16 after scaling by one power of two a tile: 2^-11 of it while it is at least 2^-28 of the tile's
+    largest step S, else half of fp16's smallest number over a scale of at least 2^14 / S: 2^-25 2^-14 S = 2^-39 S, times a
+    code of at most 15.  The weights are relative to the largest so far, so a key's share of the normalised result is off by
+    15 x 2^-39 S at most, n keys' by n times that.  A query number keeps its 8 bits while its lowest one is at least 2^-24
+    after scaling by at least 2^13 over the largest number Q, and over 16 at odd positions: down to 2^-26 Q.  Below, it is off
+    by 16 x 2^-25 x 2^-13 Q = 2^-34 Q, times a code of at most 15 and the step."""
+    from astrai_b200 import ops
+    from astrai_b200.ops import kv4
+
+    pools, table, rows, n, q, _ = _case([70, 40, 300], 4, 2, dim, seed=41)
+    used = torch.cat([table[int(r), :m] for r, m in zip(rows, n.tolist())])
+    scale = dim ** -0.5
+    far = torch.ones(dim, device="cuda")
+    far[32:64] = 2.0 ** -gap
+    k, v = _rows(410, 2, dim, seed=42), _rows(410, 2, dim, seed=43)
+    for kk, vv, qq, short in ((k, v * far, q, "value"), (k / far, v, q * far, "query")):
+        kk, vv, qq = (x.bfloat16() for x in (kk, vv, qq))
+        ops.kv4_append_(kk, vv, *pools, used)
+        o, tol = _expected(pools, table, rows, n, qq, scale)
+        out = ops.kv4_decode(qq, *pools, table, rows, n)
+        for i, length in enumerate(n.tolist()):
+            slots = table[int(rows[i]), :length].long()
+            if short == "value":
+                largest = pools[3][slots][..., 1].double().amax((0, 2)).repeat_interleave(2)  # of a kv head -> [heads]
+                tol[i] += length * 15 * 2.0 ** -39 * largest[:, None]
+            else:
+                steps = (pools[1][slots][..., 1].double().sum(-1) * 32).amax(0).repeat_interleave(2)  # sum over a row's numbers
+                off = 15 * 2.0 ** -34 * qq[i].double().abs().amax(-1) * steps * scale
+                vd = kv4.dequantize(pools[2][slots], pools[3][slots], False).double().abs().amax(0).repeat_interleave(2, 0)
+                tol[i] += 2 * (off.exp() - 1).clamp(max=1)[:, None] * vd  # p changes by a factor of at most exp(off), its sum too
+        _near(out, (o, tol))
