@@ -447,3 +447,19 @@ def test_a_captured_step_is_told_the_longest_length_a_request_can_have(model):
     assert ex.task_cache.task_alloc("a", [1, 2, 3])
     kv = ex.task_cache.bind(["a"], ex.workspace)
     assert kv.max_len == 3 and ex._padded(kv, 1, 2).max_len == 48
+
+
+def test_a_replica_cut_over_two_ranks_serves_forks_over_a_four_bit_cache(tmp_path):
+    import json
+    import os
+
+    from helpers import launch_ranks
+
+    out, root = str(tmp_path / "res"), os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code, log = launch_ranks(2, os.path.join(root, "tests", "workers", "tp_kv4.py"), ["--out", out], 29786, cwd=root)
+    assert code == 0, log
+    a, b = (json.load(open(f"{out}.{r}")) for r in range(2))
+    assert a["pool"] == b["pool"] == [[1, 16], [1, 1, 2]] * 2  # one of the two kv heads of 32 numbers each
+    assert a["greedy"] == b["greedy"] == a["alone"] and all(len(g) == 8 for g in a["greedy"])
+    assert a["sampled"] == b["sampled"] and a["sampled"][0] != a["sampled"][1]
+    assert a["chunked"] == b["chunked"] == [g for i, g in enumerate(a["alone"]) if i % 3 < 2]

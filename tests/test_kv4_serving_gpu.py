@@ -111,3 +111,144 @@ def test_a_table_whose_positions_would_pass_32_bits_is_refused():
     table = torch.empty(1, 2 ** 31 - 512, dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="table too large"):
         ops.kv4_decode(q, *pools, table, rows, torch.zeros(1, dtype=torch.int64, device="cuda"))
+
+
+# --------------------------------------------------------------------------------------------- what serving runs
+def _scheduler(model, **kw):
+    from astrai_b200.inference import InferenceScheduler
+    from test_kv4_gpu import _Tok
+
+    return InferenceScheduler(model, _Tok(), **{"max_batch_size": 8, "max_seq_len": 256, "kv_dtype": "int4", **kw})
+
+
+def _record_logits(sched, monkeypatch):
+    """Every row of logits that is sampled from, ``(task id, position in the answer, logits)`` in order."""
+    seen, plain = [], sched._executor._sample
+
+    def sample(logits, tasks, *args, **kw):
+        seen.extend((t.task_id, len(t.output_ids), row.float().clone()) for t, row in zip(tasks, logits))
+        return plain(logits, tasks, *args, **kw)
+
+    monkeypatch.setattr(sched._executor, "_sample", sample)
+    return seen
+
+
+PROMPTS = [[(7 * i + 3 * j * j) % 490 + 5 for j in range(n)] for i, n in enumerate((40, 3, 65, 130, 16))]
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_replayed_step_with_padded_rows_computes_what_the_cache_holds(paged, monkeypatch):
+    """A decode step of 5 requests in a graph of 8 rows: its logits are those of the same launches made one by one, and the
+    attention of every layer is the 64-bit one over the rows that the cache holds."""
+    from astrai_b200.ops import kv4
+    from test_kv4_gpu import _expected as expected, _model, _near
+
+    sched = _scheduler(_model(), paged=paged, page_size=16 if paged else 1)
+    ex, tc = sched._executor, sched._task_cache
+    assert sched.cuda_graph_enabled and ex._bucket(5) == 8
+    from astrai_b200.inference.task import Task
+
+    tasks = [Task(f"t{i}", list(p), 9, 0.0, 1.0, 50, 0.0, 64) for i, p in enumerate(PROMPTS)]
+    for t in tasks:
+        t.input_tokens = len(t.prompt_ids)
+        assert tc.task_alloc(t.task_id, t.prompt_ids)
+    done, tokens = ex.execute_prefill(tasks)
+    assert done == tasks
+    for t, token in zip(tasks, tokens):
+        t.output_ids.append(token)
+        t.mark_prefill_done()
+    calls, plain = [], kv4.kv4_decode
+
+    def recorded(q, *args, **kw):
+        out = plain(q, *args, **kw)
+        calls.append((q.clone(), args, out.clone(), kw["max_len"]))
+        return out
+
+    for step in range(3):
+        for t in tasks:
+            assert tc.task_extend(t.task_id, t.next_pos)
+        got = []
+        with monkeypatch.context() as patch:
+            patch.setattr(ex, "_sample", lambda logits, *a, **kw: got.append(logits.clone()) or logits.argmax(-1).tolist())
+            tokens = ex.execute_decode(tasks)  # the graph
+        ws = ex.workspace
+        with monkeypatch.context() as patch, torch.inference_mode():
+            patch.setattr(kv4, "kv4_decode", recorded)
+            kv = ex._padded(tc.bind([t.task_id for t in tasks], ws), 5, 8)  # the same step once more, launch by launch
+            ex._zero_padding(5, 8)
+            out = ex.model(input_ids=ws.input_ids[:8], kv_cache=kv, position_ids=ws.position_ids[:8], fwd="decode")["logits"]
+        assert torch.equal(got[0], out[:5])
+        lens = torch.tensor([len(p) + 1 + step for p in PROMPTS] + [0] * 3)
+        assert len(calls) == 2 * (step + 1)
+        for q, (*pools, table, rows, n), o, max_len in calls[-2:]:
+            assert torch.equal(n.cpu(), lens) and max_len == 256
+            _near(o, expected(pools, table, rows, n, q, q.shape[-1] ** -0.5))
+        ex._decode_cache = None  # the bind in between was not the executor's
+        for t, token in zip(tasks, tokens):
+            t.output_ids.append(token)
+            t.advance_kv()
+
+
+@pytest.mark.parametrize("kv_dtype", ["int4", "auto"])
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_fork_holds_its_leaders_rows_in_every_layer(paged, kv_dtype):
+    from test_kv4_gpu import _model
+
+    sched = _scheduler(_model(), paged=paged, page_size=16 if paged else 1, kv_dtype=kv_dtype, enable_cuda_graph=False)
+    tc, table, pools = sched._task_cache, sched.cache.req_pool.req_to_token, sched.cache.storage.pools()
+    assert tc.task_alloc("a", list(range(100)))
+    for t in pools:
+        t.copy_(torch.randint(1, 100, t.shape, device="cuda"))
+    before = [t.clone() for t in pools]
+    for name, length in (("b", 100), ("c", 37), ("d", 32), ("e", 1)):
+        assert tc.task_fork("a", name, length)
+        a, f = (table[tc.state(n).req_idx, :length].long() for n in ("a", name))
+        assert (a.device.type, a.numel()) == ("cuda", length)
+        for t, old in zip(pools, before):
+            assert torch.equal(t[:, f], old[:, a]) and torch.equal(t[:, a], old[:, a])
+        shared = length // 16 * 16 if paged else 0
+        assert torch.equal(a[:shared], f[:shared]) and not set(a[shared:].tolist()) & set(f[shared:].tolist())
+
+
+def _close(a, b, what):
+    """Logits of the same numbers through launches of other shapes.  Both runs round to bf16 (2^-9 of a number, either way)
+    after some 10 operations in each of 2 layers and may round each the other way: 20 x 2^-8 of the logits' size if every
+    rounding adds up; the prompt's last position sees bf16 rows in one and the codes' own numbers in the other: 2^-8 more in
+    keys and values of each layer.  That is 0.1; a wrong row, page or length gives logits of another token, 1.4."""
+    off = ((a - b).norm() / b.norm()).item()
+    assert off < 0.1, f"{what}: {off:.3f}"
+
+
+def test_forks_answer_from_their_leaders_prompt(monkeypatch):
+    from test_kv4_gpu import _model
+
+    sched = _scheduler(_model(), max_batch_size=16)
+    names = {}
+    plain = sched._task_cache.task_fork
+    monkeypatch.setattr(sched._task_cache, "task_fork", lambda a, b, n=None: names.update({b: a}) or plain(a, b, n))
+    seen = _record_logits(sched, monkeypatch)
+    answers = sched.run_batch(PROMPTS, max_tokens=6, temperature=0.0, samples_per_prompt=3)
+    assert len(answers) == 15 and all(len(a) == 6 for a in answers) and len(names) == 10
+    first = {task: row for task, n, row in seen if n == 0}
+    for fork, leader in names.items():
+        _close(first[fork], first[leader], f"{fork} of {leader}")
+    leaders = list(dict.fromkeys(names.values()))
+    for i, a in enumerate(leaders):  # the bound tells prompts apart
+        for b in leaders[:i]:
+            assert ((first[a] - first[b]).norm() / first[b].norm()).item() > 0.3
+
+
+@pytest.mark.parametrize("kv_dtype", ["int4", "auto"])
+def test_chunks_answer_as_the_whole_prompt_does(kv_dtype, monkeypatch):
+    from test_kv4_gpu import _model
+
+    model, rows = _model(), []
+    for kw in ({}, {"chunked_prefill": True, "max_prefill_tokens": 24}):
+        sched = _scheduler(model, kv_dtype=kv_dtype, **kw)
+        seen = _record_logits(sched, monkeypatch)
+        for p in PROMPTS:  # one after the other: a request's logits come in order
+            assert len(sched.run_batch([p], max_tokens=1, temperature=0.0)[0]) == 1
+        assert len(seen) == len(PROMPTS)
+        rows.append([row for _, _, row in seen])
+    for p, whole, cut in zip(PROMPTS, *rows):
+        _close(cut, whole, f"prompt of {len(p)}")
