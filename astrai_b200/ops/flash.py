@@ -82,14 +82,19 @@ def flash_attention_varlen(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
 
 def derivatives_asked(*tensors: Tensor) -> bool:
     """Whether reverse or forward mode follows what is computed from these."""
-    return any((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    recording = torch.is_grad_enabled()
+    for t in tensors:
+        if (recording and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None:
+            return True
+    return False
 
 
 def flash_attention_ragged(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, max_q: int, max_k: int,
-                           scale: float) -> Tensor:
+                           scale: float, rows_alone: bool = False) -> Tensor:
     """Causal :func:`flash_attention_varlen` of a serving step: straight to the kernel where no derivative is asked for
-    (short prompts spend more time in Python than on the GPU), with it otherwise."""
-    if derivatives_asked(q, k, v):
+    (short prompts spend more time in Python than on the GPU), with it otherwise.  ``rows_alone``: ``k`` and ``v`` were read
+    out of a 4-bit pool, through which no derivative goes."""
+    if derivatives_asked(q) if rows_alone else derivatives_asked(q, k, v):
         return flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_q, max_k, causal=True, scale=scale)
     native.require()
     return torch.ops.astrai_b200.flash_fwd(_fix(q), _fix(k), _fix(v), cu_seqlens_q.int(), cu_seqlens_k.int(), cu_seqlens_q.numel() - 1,

@@ -109,16 +109,15 @@ def read_back_pieces(kv_lens: Sequence[int], limit: int) -> List[Tuple[int, int]
 def _read_back_attention(q: Tensor, pools, cache: KVCache, q_lens, kv_lens, scale: float) -> Tensor:
     """Ragged prefill over a 4-bit pool.  The prompt's own rows are read back with the cached ones, so that a position sees
     the same numbers of a key whether its prompt ran in one chunk or in several."""
-    heads, dim = pools[0].shape[1], q.shape[-1]
-    pieces = read_back_pieces(kv_lens, READ_BACK_BYTES // (4 * heads * dim))
-    if len(pieces) == 1:
+    limit = READ_BACK_BYTES // (4 * pools[0].shape[1] * q.shape[-1])
+    if sum(kv_lens) <= limit or len(kv_lens) == 1:
         return flash.flash_attention_ragged(q, *kv4.kv4_gather(*pools, cache.kv_gather_loc), cache.qo_indptr, cache.kv_indptr,
-                                            max(q_lens), max(kv_lens), scale)
+                                            max(q_lens), max(kv_lens), scale, rows_alone=True)
     outs, q0, k0 = [], 0, 0
-    for a, b in pieces:
+    for a, b in read_back_pieces(kv_lens, limit):
         q1, k1 = q0 + sum(q_lens[a:b]), k0 + sum(kv_lens[a:b])
         outs.append(flash.flash_attention_ragged(q[q0:q1], *kv4.kv4_gather(*pools, cache.kv_gather_loc[k0:k1]), cache.qo_indptr[a:b + 1] - q0,
-                                                 cache.kv_indptr[a:b + 1] - k0, max(q_lens[a:b]), max(kv_lens[a:b]), scale))
+                                                 cache.kv_indptr[a:b + 1] - k0, max(q_lens[a:b]), max(kv_lens[a:b]), scale, rows_alone=True))
         q0, k0 = q1, k1
     return torch.cat(outs)
 
@@ -126,8 +125,10 @@ def _read_back_attention(q: Tensor, pools, cache: KVCache, q_lens, kv_lens, scal
 def _one_position_each(q: Tensor, cache: KVCache, q_lens) -> bool:
     """A prefill that the decode kernel answers: one query of each request, no derivative asked for.  Heads of 128, 8 forks of
     4096 positions (16 / 4 heads): 40 us, and 90 us with the rows read back; 64 of 16384 (32 / 8): 0.32 and 4.9 ms."""
+    if max(q_lens) != 1:
+        return False
     hkv = cache.k_buffer.shape[2]
-    return (max(q_lens) == 1 and len(q_lens) == q.shape[0] and q.shape[1] % hkv == 0 and 1 <= q.shape[1] // hkv <= 8
+    return (len(q_lens) == q.shape[0] and q.shape[1] % hkv == 0 and 1 <= q.shape[1] // hkv <= 8
             and cache.seq_lens.dtype == torch.int64 and cache.req_pool_indices.dtype == torch.int32
             and not flash.derivatives_asked(q))
 
