@@ -93,12 +93,15 @@ def flash_attention_ragged(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor
                            scale: float, rows_alone: bool = False) -> Tensor:
     """Causal :func:`flash_attention_varlen` of a serving step: straight to the kernel where no derivative is asked for
     (short prompts spend more time in Python than on the GPU), with it otherwise.  ``rows_alone``: ``k`` and ``v`` were read
-    out of a 4-bit pool, through which no derivative goes."""
+    out of a 4-bit pool: packed, and no derivative goes through them."""
     if derivatives_asked(q) if rows_alone else derivatives_asked(q, k, v):
         return flash_attention_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_q, max_k, causal=True, scale=scale)
     native.require()
-    return torch.ops.astrai_b200.flash_fwd(_fix(q), _fix(k), _fix(v), cu_seqlens_q.int(), cu_seqlens_k.int(), cu_seqlens_q.numel() - 1,
-                                           0, 0, int(max_q), True, float(scale))[0]
+    cu_q = cu_seqlens_q if cu_seqlens_q.dtype is torch.int32 else cu_seqlens_q.int()
+    cu_k = cu_seqlens_k if cu_seqlens_k.dtype is torch.int32 else cu_seqlens_k.int()
+    if not rows_alone:
+        k, v = _fix(k), _fix(v)
+    return torch.ops.astrai_b200.flash_fwd(_fix(q), k, v, cu_q, cu_k, cu_q.numel() - 1, 0, 0, int(max_q), True, float(scale))[0]
 
 
 PAGED_PAGE_SIZES = (8, 16, 32, 64)

@@ -142,7 +142,7 @@ def kv4_decode(q: Tensor, k_codes: Tensor, k_meta: Tensor, v_codes: Tensor, v_me
 
     The keys of the whole batch are spread evenly over the GPU, whatever the lengths.  ``max_len``: the longest length, when
     the host knows it (0: the table's width) - it sizes the launch, a longer request is served all the same.  ``workspace``:
-    see :func:`kv4_decode_workspace`; without one the call allocates its own scratch."""
+    see :func:`kv4_decode_workspace`; without one the call allocates its own scratch.  On CUDA no derivative is recorded."""
     scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
     if k_codes.is_cuda:
         o_part, ml_part, counters = workspace if workspace is not None else (None, None, None)

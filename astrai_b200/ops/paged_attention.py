@@ -107,8 +107,8 @@ def read_back_pieces(kv_lens: Sequence[int], limit: int) -> List[Tuple[int, int]
 
 
 def _read_back_attention(q: Tensor, pools, cache: KVCache, q_lens, kv_lens, scale: float) -> Tensor:
-    """Ragged prefill over a 4-bit pool.  The prompt's own rows are read back with the cached ones, so that a position sees
-    the same numbers of a key whether its prompt ran in one chunk or in several."""
+    """Ragged prefill over a 4-bit pool.  The prompt's own rows are read back with the cached ones, so that the positions of a
+    chunk see the same numbers of a key wherever the prompt was cut."""
     limit = READ_BACK_BYTES // (4 * pools[0].shape[1] * q.shape[-1])
     if sum(kv_lens) <= limit or len(kv_lens) == 1:
         return flash.flash_attention_ragged(q, *kv4.kv4_gather(*pools, cache.kv_gather_loc), cache.qo_indptr, cache.kv_indptr,
@@ -123,10 +123,8 @@ def _read_back_attention(q: Tensor, pools, cache: KVCache, q_lens, kv_lens, scal
 
 
 def _one_position_each(q: Tensor, cache: KVCache, q_lens) -> bool:
-    """A prefill that the decode kernel answers: one query of each request, no derivative asked for.  Heads of 128, 8 forks of
+    """A prefill of at most one query of each request that the decode kernel answers: one of each, no derivative asked for.  Heads of 128, 8 forks of
     4096 positions (16 / 4 heads): 40 us, and 90 us with the rows read back; 64 of 16384 (32 / 8): 0.32 and 4.9 ms."""
-    if max(q_lens) != 1:
-        return False
     hkv = cache.k_buffer.shape[2]
     return (len(q_lens) == q.shape[0] and q.shape[1] % hkv == 0 and 1 <= q.shape[1] // hkv <= 8
             and cache.seq_lens.dtype == torch.int64 and cache.req_pool_indices.dtype == torch.int32
@@ -169,7 +167,7 @@ def cached_attention(q: Tensor, k: Tensor, v: Tensor, kv_cache: KVCache, layer_i
     page = getattr(kv_cache, "page_size", 1) or 1
     if pools is not None:
         if native_on and attn_mask is None and fwd == "prefill" and q.is_cuda and q.dtype == torch.bfloat16:
-            if _one_position_each(q, kv_cache, q_lens):
+            if max(q_lens) == 1 and _one_position_each(q, kv_cache, q_lens):
                 return kv4.kv4_decode(q, *pools, kv_cache.req_to_token, kv_cache.req_pool_indices, kv_cache.seq_lens, scale=scale,
                                       max_len=max(kv_lens))
             if kv_cache.kv_gather_loc is not None and kv_cache.qo_indptr is not None and q.shape[-1] in flash.SUPPORTED_HEAD_DIMS:
