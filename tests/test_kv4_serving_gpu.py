@@ -252,3 +252,29 @@ def test_chunks_answer_as_the_whole_prompt_does(kv_dtype, monkeypatch):
         rows.append([row for _, _, row in seen])
     for p, whole, cut in zip(PROMPTS, *rows):
         _close(cut, whole, f"prompt of {len(p)}")
+
+
+@pytest.mark.parametrize("counts", [[5, 3], [1, 1]])
+def test_no_derivative_is_dropped_on_the_way_through_a_four_bit_cache(counts):
+    import torch.autograd.forward_ad as fwAD
+
+    from astrai_b200 import ops
+
+    heads, kv_heads, dim, lens = 4, 2, 64, [70, 40]
+    pool, tc, ws = _cached(lens, heads, kv_heads, dim)
+    kv = tc.bind(["t0", "t1"], ws, start_positions=[n - c for n, c in zip(lens, counts)])
+    q, k, v = (_rows(sum(counts), h, dim, seed=50 + h) for h in (heads, kv_heads, kv_heads))
+    plain = ops.attention(q, k, v, kv, 0, None, True, "prefill")
+    qg = q.clone().requires_grad_()
+    out = ops.attention(qg, k, v, kv, 0, None, True, "prefill")
+    o, tol = _expected(pool, kv, q, counts, lens, 1, dim ** -0.5)
+    for got in (plain, out.detach()):
+        assert ((got[counts[0]:].double() - o).abs() <= tol).all()
+    out.float().sum().backward()
+    assert torch.isfinite(qg.grad).all() and qg.grad.abs().max() > 0
+    with fwAD.dual_level():
+        try:
+            out = ops.attention(fwAD.make_dual(q, torch.randn_like(q)), k, v, kv, 0, None, True, "prefill")
+        except (NotImplementedError, RuntimeError):
+            return
+        assert fwAD.unpack_dual(out).tangent is not None
